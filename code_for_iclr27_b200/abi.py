@@ -75,6 +75,17 @@ class Arena(ctypes.Structure):
                 ("capacity", I64), ("dimension", I64), ("dtype", I32)]
 
 
+class Pages(ctypes.Structure):
+    """lrk_pages (include/lrk.h)."""
+    _fields_ = [("keys", P), ("values", P), ("key_scales", P), ("value_scales", P), ("positions", P), ("pages", I64),
+                ("page_size", I64), ("dimension", I64), ("group", I64), ("dtype", I32)]
+
+
+class Rows(ctypes.Structure):
+    """lrk_rows (include/lrk.h)."""
+    _fields_ = [("data", P), ("token_stride", I64), ("head_stride", I64)]
+
+
 SIGNATURES = {
     "lrk_last_error": (ctypes.c_char_p, []),
     "lrk_version": (I32, []),
@@ -119,6 +130,12 @@ SIGNATURES = {
     "lrk_arena_compact_positions": (I32, [ctypes.POINTER(Arena), P, I64, P, P, P]),
     "lrk_arena_evict": (I32, [ctypes.POINTER(Arena), P, P, I64, P, P]),
     "lrk_merge_plan": (I32, [ctypes.POINTER(PlanLayer), I64, I64, P, P]),
+    "lrk_paged_append": (I32, [ctypes.POINTER(Pages), P, I64, I64, P, I64, I64, P, I64, ctypes.POINTER(Rows),
+                               ctypes.POINTER(Rows), P, P, I64, I64, I32, ctypes.POINTER(Rows), I64, P, I32, P, P]),
+    "lrk_paged_attention_workspace_bytes": (SIZE, []),
+    "lrk_paged_attention": (I32, [ctypes.POINTER(Pages), P, I64, I64, P, I64, I64, P, I64, ctypes.POINTER(Rows), I64,
+                                  F, I32, P, P, I32, P, SIZE, P, P]),
+    "lrk_paged_read": (I32, [ctypes.POINTER(Pages), P, I64, I64, P, P, I64, I64, P, P, P, I32, P, P]),
     "lrk_arena_insert": (I32, [ctypes.POINTER(Arena), P, I64, P, P, I32, P, P]),
 }
 

@@ -8,7 +8,10 @@
 // scores_from_keys, project_values, logits and logits_heads (scoring); compact_layers and
 // merge_layers (eviction and recall over several layers in one call);
 // select_histogram and select_pick (layer-group selection across GPUs);
-// arena_append and arena_compact (the gapped per-head KV arena).
+// arena_append and arena_compact (the gapped per-head KV arena); paged_append,
+// paged_attention and paged_read (the paged cache).
+#include <algorithm>
+#include <optional>
 #include <vector>
 
 #include "shim_common.h"
@@ -807,6 +810,193 @@ void arena_append_into(torch::Tensor keys, torch::Tensor values, torch::Tensor p
                                 reinterpret_cast<unsigned int *>(flag.data_ptr<int32_t>()), current_stream()));
 }
 
+// ------------------------------------------------------------ paged cache
+
+// The pages of one cache (lrk_pages): keys, values [pages, page_size, D] of
+// one 16-bit type, or uint8 [pages, page_size, D / 2] with float16 scales
+// [pages, page_size, D / group, 2].
+lrk_pages pages_of(const torch::Tensor &keys, const torch::Tensor &values, const torch::Tensor &positions,
+                   const std::optional<torch::Tensor> &key_scales, const std::optional<torch::Tensor> &value_scales) {
+  for (const auto &tensor : {keys, values, positions}) check_cuda(tensor, keys);
+  TORCH_CHECK(keys.dim() == 3 && keys.sizes() == values.sizes() && keys.scalar_type() == values.scalar_type(),
+              "pages: keys/values must be [pages, page_size, channels] of one dtype");
+  TORCH_CHECK(positions.scalar_type() == at::kFloat && positions.dim() == 2 && positions.size(0) == keys.size(0) &&
+                  positions.size(1) == keys.size(1),
+              "pages: positions must be float32 [pages, page_size]");
+  TORCH_CHECK(key_scales.has_value() == value_scales.has_value(), "pages: scales for both keys and values, or neither");
+  lrk_pages p{};
+  p.keys = keys.data_ptr();
+  p.values = values.data_ptr();
+  p.positions = positions.data_ptr<float>();
+  p.pages = keys.size(0);
+  p.page_size = keys.size(1);
+  p.dimension = keys.size(2);
+  if (key_scales.has_value()) {
+    TORCH_CHECK(keys.scalar_type() == at::kByte, "pages: 4-bit codes must be uint8");
+    p.dimension = 2 * keys.size(2);
+    for (const auto *scales : {&*key_scales, &*value_scales}) {
+      check_cuda(*scales, keys);
+      TORCH_CHECK(scales->scalar_type() == at::kHalf && scales->dim() == 4 && scales->size(0) == keys.size(0) &&
+                      scales->size(1) == keys.size(1) && scales->size(2) >= 1 && scales->size(3) == 2 &&
+                      p.dimension % scales->size(2) == 0 && scales->sizes() == key_scales->sizes(),
+                  "pages: scales must be float16 [pages, page_size, D / group, 2]");
+    }
+    p.group = p.dimension / key_scales->size(2);
+    p.key_scales = key_scales->data_ptr();
+    p.value_scales = value_scales->data_ptr();
+  } else {
+    TORCH_CHECK(keys.scalar_type() == at::kHalf || keys.scalar_type() == at::kBFloat16,
+                "pages: rows must be float16 or bfloat16, or 4-bit codes with scales");
+    p.dtype = dtype_code(keys.scalar_type());
+  }
+  return p;
+}
+
+void check_table(const torch::Tensor &table, const torch::Tensor &pages) {
+  TORCH_CHECK(table.is_cuda() && table.device() == pages.device(), "CUDA devices differ");
+  TORCH_CHECK(table.scalar_type() == at::kInt && table.dim() == 2 && (table.size(1) <= 1 || table.stride(1) == 1) &&
+                  (table.size(0) <= 1 || table.stride(0) >= table.size(1)),
+              "page table must be int32 [slots, pages of a slot] with contiguous rows");
+}
+
+int64_t table_stride(const torch::Tensor &table) {
+  return table.size(0) > 1 ? table.stride(0) : std::max<int64_t>(table.size(1), 1);
+}
+
+void check_int32(const torch::Tensor &tensor, const torch::Tensor &pages, int64_t count, const char *message) {
+  check_cuda(tensor, pages);
+  TORCH_CHECK(tensor.scalar_type() == at::kInt && tensor.numel() == count, message);
+}
+
+// A [tokens, heads, D] tensor as lrk_rows: its own strides where the kernels'
+// 16-byte vectors fit them, a contiguous copy otherwise (kept in `copy`).
+lrk_rows rows_of(const torch::Tensor &tensor, torch::Tensor &copy) {
+  const bool fits = tensor.stride(2) == 1 && tensor.stride(0) % 8 == 0 && tensor.stride(1) % 8 == 0 &&
+                    reinterpret_cast<uintptr_t>(tensor.data_ptr()) % 16 == 0;
+  copy = fits ? tensor : tensor.clone(at::MemoryFormat::Contiguous);
+  return lrk_rows{copy.data_ptr(), copy.stride(0), copy.stride(1)};
+}
+
+void check_rows(const torch::Tensor &rows, const torch::Tensor &pages, int64_t dimension, const char *message) {
+  TORCH_CHECK(rows.is_cuda() && rows.device() == pages.device(), "CUDA devices differ");
+  TORCH_CHECK(rows.dim() == 3 && rows.size(1) >= 1 && rows.size(2) == dimension &&
+                  (rows.scalar_type() == at::kHalf || rows.scalar_type() == at::kBFloat16),
+              message);
+}
+
+// Rotated rows into the pages (lrk_paged_append).  Returns the rotated
+// queries, if any.
+std::optional<torch::Tensor> paged_append(torch::Tensor keys, torch::Tensor values, torch::Tensor positions,
+                                          std::optional<torch::Tensor> key_scales,
+                                          std::optional<torch::Tensor> value_scales, torch::Tensor table,
+                                          torch::Tensor lengths, torch::Tensor new_keys, torch::Tensor new_values,
+                                          torch::Tensor new_positions, torch::Tensor token_starts, torch::Tensor flag,
+                                          std::optional<torch::Tensor> rotary, bool interleaved,
+                                          std::optional<torch::Tensor> queries) {
+  const lrk_pages p = pages_of(keys, values, positions, key_scales, value_scales);
+  check_table(table, keys);
+  check_rows(new_keys, keys, p.dimension, "new rows must be float16 or bfloat16 [tokens, heads, D]");
+  check_rows(new_values, keys, p.dimension, "new rows must be float16 or bfloat16 [tokens, heads, D]");
+  const int64_t tokens = new_keys.size(0), heads = new_keys.size(1);
+  TORCH_CHECK(new_values.sizes() == new_keys.sizes() && new_values.scalar_type() == new_keys.scalar_type(),
+              "new keys and values differ in shape or dtype");
+  TORCH_CHECK(table.size(0) % heads == 0, "page table must have sequences x heads rows");
+  const int64_t sequences = table.size(0) / heads;
+  check_int32(lengths, keys, table.size(0), "lengths must be int32 [slots]");
+  check_int32(token_starts, keys, sequences + 1, "token starts must be int32 [sequences + 1]");
+  check_cuda(new_positions, keys);
+  check_cuda(flag, keys);
+  TORCH_CHECK(new_positions.scalar_type() == at::kLong && new_positions.numel() == tokens,
+              "positions must be int64 [tokens]");
+  TORCH_CHECK(flag.scalar_type() == at::kInt && flag.numel() >= 1, "flag must be int32");
+  if (rotary.has_value()) {
+    check_cuda(*rotary, keys);
+    TORCH_CHECK(rotary->scalar_type() == at::kFloat && rotary->dim() == 2 && rotary->size(1) >= 1,
+                "rotary table must be float32 [positions, rotary dimension]");
+  }
+  c10::cuda::CUDAGuard guard(keys.device());
+  std::optional<torch::Tensor> rotated;
+  lrk_rows query_rows{};
+  torch::Tensor key_copy, value_copy, query_copy;
+  int64_t query_heads = 0;
+  if (queries.has_value()) {
+    check_rows(*queries, keys, p.dimension, "queries must be float16 or bfloat16 [tokens, heads, D]");
+    TORCH_CHECK(queries->size(0) == tokens && queries->scalar_type() == new_keys.scalar_type(),
+                "queries must have the new rows' tokens and dtype");
+    query_heads = queries->size(1);
+    query_rows = rows_of(*queries, query_copy);
+    rotated = torch::empty({tokens, query_heads, p.dimension}, queries->options());
+  }
+  const lrk_rows key_rows = rows_of(new_keys, key_copy), value_rows = rows_of(new_values, value_copy);
+  check_status(lrk_paged_append(
+      &p, table.data_ptr<int32_t>(), table_stride(table), table.size(1), lengths.data_ptr<int32_t>(), sequences, heads,
+      token_starts.data_ptr<int32_t>(), tokens, &key_rows, &value_rows, new_positions.data_ptr<int64_t>(),
+      rotary.has_value() ? rotary->data_ptr<float>() : nullptr, rotary.has_value() ? rotary->size(0) : 0,
+      rotary.has_value() ? rotary->size(1) : 0, interleaved, queries.has_value() ? &query_rows : nullptr, query_heads,
+      rotated.has_value() ? rotated->data_ptr() : nullptr, dtype_code(new_keys.scalar_type()),
+      reinterpret_cast<unsigned int *>(flag.data_ptr<int32_t>()), current_stream()));
+  return rotated;
+}
+
+// Attention over the pages (lrk_paged_attention): (out [tokens, query heads,
+// D], lse float32 [tokens, query heads]).
+std::tuple<torch::Tensor, torch::Tensor> paged_attention(
+    torch::Tensor keys, torch::Tensor values, torch::Tensor positions, std::optional<torch::Tensor> key_scales,
+    std::optional<torch::Tensor> value_scales, torch::Tensor table, torch::Tensor lengths, torch::Tensor queries,
+    torch::Tensor token_starts, torch::Tensor workspace, torch::Tensor flag, double scale, bool causal) {
+  const lrk_pages p = pages_of(keys, values, positions, key_scales, value_scales);
+  check_table(table, keys);
+  check_rows(queries, keys, p.dimension, "queries must be float16 or bfloat16 [tokens, heads, D]");
+  check_cuda(token_starts, keys);
+  check_cuda(workspace, keys);
+  check_cuda(flag, keys);
+  const int64_t sequences = token_starts.numel() - 1, tokens = queries.size(0), query_heads = queries.size(1);
+  check_int32(token_starts, keys, sequences + 1, "token starts must be int32 [sequences + 1]");
+  TORCH_CHECK(sequences >= 0 && (sequences == 0 ? table.size(0) == 0 : table.size(0) % sequences == 0),
+              "page table must have sequences x heads rows");
+  const int64_t heads = sequences > 0 ? table.size(0) / sequences : 1;
+  check_int32(lengths, keys, table.size(0), "lengths must be int32 [slots]");
+  TORCH_CHECK(flag.scalar_type() == at::kInt && flag.numel() >= 1, "flag must be int32");
+  c10::cuda::CUDAGuard guard(keys.device());
+  auto out = torch::empty({tokens, query_heads, p.dimension}, queries.options());
+  auto lse = torch::empty({tokens, query_heads}, queries.options().dtype(at::kFloat));
+  torch::Tensor copy;
+  const lrk_rows rows = rows_of(queries, copy);
+  check_status(lrk_paged_attention(&p, table.data_ptr<int32_t>(), table_stride(table), table.size(1),
+                                   lengths.data_ptr<int32_t>(), sequences, heads, token_starts.data_ptr<int32_t>(),
+                                   tokens, &rows, query_heads, static_cast<float>(scale), causal, out.data_ptr(),
+                                   lse.data_ptr<float>(), dtype_code(queries.scalar_type()), workspace.data_ptr(),
+                                   workspace.nbytes(), reinterpret_cast<unsigned int *>(flag.data_ptr<int32_t>()),
+                                   current_stream()));
+  return {out, lse};
+}
+
+// Rows of the pages in the packed layout (lrk_paged_read): (keys, values
+// [rows, D] of `dtype`, positions float32 [rows]).
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> paged_read(
+    torch::Tensor keys, torch::Tensor values, torch::Tensor positions, std::optional<torch::Tensor> key_scales,
+    std::optional<torch::Tensor> value_scales, torch::Tensor table, torch::Tensor first_rows, torch::Tensor row_starts,
+    int64_t rows, at::ScalarType dtype, torch::Tensor flag) {
+  const lrk_pages p = pages_of(keys, values, positions, key_scales, value_scales);
+  check_table(table, keys);
+  const int64_t slots = table.size(0);
+  check_int32(first_rows, keys, slots, "first rows must be int32 [slots]");
+  check_int32(row_starts, keys, slots + 1, "row starts must be int32 [slots + 1]");
+  check_cuda(flag, keys);
+  TORCH_CHECK(flag.scalar_type() == at::kInt && flag.numel() >= 1, "flag must be int32");
+  TORCH_CHECK(rows >= 0, "negative row count");
+  c10::cuda::CUDAGuard guard(keys.device());
+  auto out_keys = torch::empty({rows, p.dimension}, keys.options().dtype(dtype));
+  auto out_values = torch::empty({rows, p.dimension}, keys.options().dtype(dtype));
+  auto out_positions = torch::empty({rows}, positions.options());
+  check_status(lrk_paged_read(&p, table.data_ptr<int32_t>(), table_stride(table), table.size(1),
+                              first_rows.data_ptr<int32_t>(), row_starts.data_ptr<int32_t>(), slots, rows,
+                              out_keys.data_ptr(), out_values.data_ptr(), out_positions.data_ptr<float>(),
+                              dtype_code(dtype), reinterpret_cast<unsigned int *>(flag.data_ptr<int32_t>()),
+                              current_stream()));
+  return {out_keys, out_values, out_positions};
+}
+
 // Recall merge plans of several layers on the device (recall/planning.py:34-52).
 // Per layer: positions (f32, the layer's [rows] or [rows, 1]), head_starts
 // (int32 [heads + 1]), recalled positions (f32, sorted by (head, position)),
@@ -971,6 +1161,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, module) {
   module.def("arena_compact_positions", &arena_compact_positions);
   module.def("arena_evict", &arena_evict);
   module.def("arena_append_into", &arena_append_into);
+  module.def("paged_append", &paged_append);
+  module.def("paged_attention", &paged_attention);
+  module.def("paged_read", &paged_read);
   module.def("merge_plan", &merge_plan);
   module.def("reinsert_layers", &reinsert_layers);
 }

@@ -494,6 +494,95 @@ int lrk_arena_insert(const lrk_arena *arena, const int64_t *plan, int64_t touche
 int lrk_arena_evict(const lrk_arena *arena, const int64_t *heads, const float *removed_positions, int64_t count,
                     unsigned int *error, lrk_stream_t stream);
 
+/* -------------------------------------------------------- paged cache */
+
+/* A cache in pages: a page holds page_size rows of ONE slot (one KV head of
+ * one sequence; slot = sequence x heads + head), so the slots of a sequence
+ * can hold different numbers of rows.  Row r of a slot lies in page
+ * table[slot][r / page_size], place r % page_size; table is i32 [slots,
+ * table_width] with a row stride of table_stride, device memory.
+ *   group == 0: keys, values [pages, page_size, dimension] of dtype (f16, bf16);
+ *   group  > 0: keys, values are 4-bit codes u8 [pages, page_size, dimension/2]
+ *     (channel 2j in the low half of byte j) and key_scales, value_scales are
+ *     f16 [pages, page_size, dimension/group, 2], a (scale, offset) pair per
+ *     group of channels; a channel's value is offset + scale (code - 8).
+ * positions f32 [pages, page_size]: each row's logical position.  All device
+ * memory, rows and scales 16-byte aligned; page_size 16, 32, 64 or 128;
+ * dimension 64 or 128; group 32, 64 or 128, at most dimension.
+ * No counterpart in the reference, whose cache is packed
+ * (src/lazy_recall/cache.py:16-265) and whose attention is FlashAttention
+ * over it (src/lazy_recall/attention.py:15-35).
+ *
+ * The operators OR bits into *flag (device, required): 1 a length, row or
+ * page id outside the table or the pages (that row is not touched), 2 a
+ * position outside the rotary table (that token's keys and queries are not
+ * written), 4 a bounded wait inside a kernel ran out. */
+typedef struct lrk_pages {
+  void *keys;
+  void *values;
+  void *key_scales;
+  void *value_scales;
+  float *positions;
+  int64_t pages;
+  int64_t page_size;
+  int64_t dimension;
+  int64_t group;
+  int dtype; /* of 16-bit rows; not used with group > 0 */
+} lrk_pages;
+
+/* Rows [tokens, heads, dimension] with strides in elements (multiples of 8),
+ * a row's channels contiguous, 16-byte aligned. */
+typedef struct lrk_rows {
+  const void *data;
+  int64_t token_stride;
+  int64_t head_stride;
+} lrk_rows;
+
+/* Appends each sequence's new rows: token i of sequence s, i counted from
+ * token_starts[s] (i32 [sequences + 1], device, ascending from 0 to tokens),
+ * becomes row lengths[slot] - n_s + i of its slots; lengths (i32 [sequences x
+ * heads], device) are the lengths AFTER the append and are not changed.
+ * Keys and, if query_heads > 0, queries (written to out_queries, contiguous
+ * [tokens, query_heads, dimension]) are rotated on the way by row
+ * positions[token] (i64 [tokens]) of rotary (f32 [rotary_positions,
+ * rotary_dim]: rotary_dim / 2 cosines, then as many sines), over their first
+ * rotary_dim channels: pairs (j, j + rotary_dim/2), or (2j, 2j + 1) with
+ * interleaved.  rotary_dim 0: no rotation.  Rows are rounded to the pages'
+ * 16-bit type, or quantised per group: scale = f16((max - min)/15), offset =
+ * f16(min + 8 scale), code = rint((x - offset)/scale) + 8 held to 0..15.  A
+ * group that is not finite, or passes f16's range, is held as NaN. */
+int lrk_paged_append(const lrk_pages *pages, const int32_t *table, int64_t table_stride, int64_t table_width,
+                     const int32_t *lengths, int64_t sequences, int64_t heads, const int32_t *token_starts,
+                     int64_t tokens, const lrk_rows *keys, const lrk_rows *values, const int64_t *positions,
+                     const float *rotary, int64_t rotary_positions, int64_t rotary_dim, int interleaved,
+                     const lrk_rows *queries, int64_t query_heads, void *out_queries, int dtype, unsigned int *flag,
+                     lrk_stream_t stream);
+
+/* Attention of each sequence's tokens over its slots: query head h reads KV
+ * head h / (query_heads / heads); with causal, token i of n_s sees rows
+ * r <= lengths[slot] - n_s + i, without it every row below lengths[slot].
+ * out [tokens, query_heads, dimension] of dtype = softmax(scale q k) v, lse
+ * f32 [tokens, query_heads] = log sum exp(scale q k); a query without a
+ * visible row gives 0 and -inf.  What lies in pages beyond a slot's length is
+ * never used.  16-bit pages and queries share one type.
+ * workspace: lrk_paged_attention_workspace_bytes() bytes, 16-byte aligned,
+ * zeroed once by the caller and left zeroed where it must be; calls that may
+ * overlap need one each. */
+size_t lrk_paged_attention_workspace_bytes(void);
+int lrk_paged_attention(const lrk_pages *pages, const int32_t *table, int64_t table_stride, int64_t table_width,
+                        const int32_t *lengths, int64_t sequences, int64_t heads, const int32_t *token_starts,
+                        int64_t tokens, const lrk_rows *queries, int64_t query_heads, float scale, int causal,
+                        void *out, float *lse, int dtype, void *workspace, size_t workspace_bytes,
+                        unsigned int *flag, lrk_stream_t stream);
+
+/* Rows back in the packed layout: row j of slot s's row_starts[s+1] -
+ * row_starts[s] rows (i32 [slots + 1], device, from 0 to rows) is the slot's
+ * row first_rows[s] + j; keys, values [rows, dimension] of dtype (f16, bf16 or
+ * f32: the values that the rows stand for), positions f32 [rows]. */
+int lrk_paged_read(const lrk_pages *pages, const int32_t *table, int64_t table_stride, int64_t table_width,
+                   const int32_t *first_rows, const int32_t *row_starts, int64_t slots, int64_t rows, void *keys,
+                   void *values, float *positions, int dtype, unsigned int *flag, lrk_stream_t stream);
+
 /* ---------------------------------------------- layer-group selection */
 
 /* The request-wide "k smallest raw scores" when one request's layers are
