@@ -436,14 +436,14 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() {
 }
 
 // bf16 matrix [rows_total, columns] with a row stride of `stride` elements;
-// boxes of box_columns x 128 rows.
+// boxes of box_columns x box_rows.
 int make_map(CUtensorMap *map, const void *data, int64_t rows_total, int64_t columns, int64_t stride,
-             uint32_t box_columns, CUtensorMapSwizzle swizzle) {
+             uint32_t box_columns, CUtensorMapSwizzle swizzle, uint32_t box_rows) {
   auto encode = encode_tiled();
   if (encode == nullptr) return fail(LRK_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   const cuuint64_t sizes[2] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(rows_total)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * 2};
-  const cuuint32_t box[2] = {box_columns, kRows};
+  const cuuint32_t box[2] = {box_columns, box_rows};
   const cuuint32_t element_strides[2] = {1, 1};
   const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(data), sizes, strides, box,
                             element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,

@@ -167,9 +167,10 @@ __device__ __forceinline__ uint32_t swizzled(int r, int c) {
 }
 
 // Host: tensor map of a bf16 matrix [rows_total, columns] with a row stride of
-// `stride` elements; boxes of box_columns x 128 rows (logits_tc.cu).
+// `stride` elements; boxes of box_columns x box_rows (logits_tc.cu).  A copy
+// moves bits, so the map serves any 16-bit type.
 int make_map(CUtensorMap *map, const void *data, int64_t rows_total, int64_t columns, int64_t stride,
-             uint32_t box_columns, CUtensorMapSwizzle swizzle);
+             uint32_t box_columns, CUtensorMapSwizzle swizzle, uint32_t box_rows = kRows);
 
 }  // namespace tc
 }  // namespace lrk
