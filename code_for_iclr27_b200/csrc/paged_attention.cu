@@ -51,6 +51,21 @@ constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kMinTiles = kWarps;  // tiles per block, at least
 constexpr int kCounters = 4096;    // workspace: arrival counters, then partial results
 
+// Division by a number that the host knows: n / d for n below 2^31 as a
+// product (Granlund and Montgomery's round-up method).
+struct Divider {
+  uint32_t multiplier, shift;
+  static Divider of(uint32_t d) {
+    Divider r{0, 0};
+    while ((uint64_t{1} << r.shift) < d) ++r.shift;
+    r.multiplier = static_cast<uint32_t>(((((uint64_t{1} << r.shift) - d) << 32) / d) + 1);
+    return r;
+  }
+  __device__ __forceinline__ int32_t operator()(int32_t n) const {
+    return static_cast<int32_t>((__umulhi(static_cast<uint32_t>(n), multiplier) + static_cast<uint32_t>(n)) >> shift);
+  }
+};
+
 struct AttentionParam {
   Pages pages;
   const int32_t *table;
@@ -62,6 +77,7 @@ struct AttentionParam {
   const void *queries;
   int64_t query_token, query_head;
   int heads, groups;
+  Divider by_heads, by_groups;
   float scale_log2;
   bool causal;
   void *out;
@@ -79,32 +95,41 @@ struct Layout {
   static constexpr int kRows = 8 * NT;  // query rows per block
   static constexpr int kCodes = kTile * kRowBytes, kScales = kTile * kScaleBytes;
   static constexpr int kStage = 2 * (kCodes + kScales);  // key rows, key scales, value rows, value scales
-  static constexpr int kStages = GROUP ? 10 : (D == 128 ? 4 : 8);
   static constexpr int kPitch = D + 4;
   static constexpr int kScratch = kWarps * 8 * kPitch * 4;
   static constexpr int kQuery = NT * (D / 16) * 32 * 8;
+  // Blocks on an SM, by registers (NT = 1: 96 a thread for 4-bit rows, 128 for
+  // 16-bit ones), and as many stages as their share of shared memory holds.
+  static constexpr int kBlocksPerSm = NT == 1 ? (GROUP ? 4 : D == 128 ? 2 : 3) : (NT == 2 ? 2 : 1);
+  static constexpr int kControl = 256;  // bytes of Control
+  static constexpr int kFixed = kScratch + kQuery + kGroups * kRows * 8 + kRows * 4 + 2 * kWarps * kRows * 4 + 2 * 16 * 8 +
+                                kControl;
+  static constexpr int kFit = ((232448 / kBlocksPerSm - 1024) / 128 * 128 - kFixed) / kStage;
+  // A multiple of the warps, so that a stage always falls to the same warp: it
+  // has then seen the stage's last phase end, and a parity names one phase.
+  static constexpr int kStages = (kFit > 12 ? 12 : kFit) / kWarps * kWarps;
   // After the stages: scratch, query fragments, group sums, factors, maxima and sums, barriers.
   static constexpr int kScratchAt = kStages * kStage;
   static constexpr int kQueryAt = kScratchAt + kScratch;
   static constexpr int kSumsAt = kQueryAt + kQuery;
-  static constexpr int kFactorAt = kSumsAt + kGroups * kRows * 4;
+  static constexpr int kFactorAt = kSumsAt + kGroups * kRows * 8;
   static constexpr int kStatsAt = kFactorAt + kRows * 4;
   static constexpr int kBarriersAt = kStatsAt + 2 * kWarps * kRows * 4;
-  static constexpr int kBytes = kBarriersAt + 2 * kStages * 8 + 64 + 1024;
-  static constexpr int kBlocksPerSm = NT == 1 ? 3 : (NT == 2 ? 2 : 1);
+  static constexpr int kBytes = kBarriersAt + 2 * kStages * 8 + kControl;
+  static_assert(kStages >= kWarps, "every warp needs a stage of its own");
 };
 
 __device__ __forceinline__ void mma(const __half *, float *d, const uint32_t *a, uint32_t b0, uint32_t b1,
                                     const float *c) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 __device__ __forceinline__ void mma(const __nv_bfloat16 *, float *d, const uint32_t *a, uint32_t b0, uint32_t b1,
                                     const float *c) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
@@ -113,7 +138,7 @@ __device__ __forceinline__ void mma(const __nv_bfloat16 *, float *d, const uint3
 // columns of S^T (query rows) become the rows that P's B operand wants.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
   return y;
 }
 
@@ -126,6 +151,10 @@ __device__ __forceinline__ uint32_t pack(const __nv_bfloat16 *, float lo, float 
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+__device__ __forceinline__ uint32_t shared_address(const void *p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -133,23 +162,19 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 
 template <int WORDS>
-__device__ __forceinline__ void load_words(uint32_t address, uint32_t *w) {
-  if constexpr (WORDS == 4)
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(address));
-  else if constexpr (WORDS == 2)
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(address));
-  else
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(address));
+__device__ __forceinline__ void load_words(const uint8_t *from, uint32_t *w) {
+  if constexpr (WORDS == 4) {
+    const uint4 x = *reinterpret_cast<const uint4 *>(from);
+    w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+  } else if constexpr (WORDS == 2) {
+    const uint2 x = *reinterpret_cast<const uint2 *>(from);
+    w[0] = x.x, w[1] = x.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t *>(from);
+  }
 }
-__device__ __forceinline__ uint32_t load_short(uint32_t address) {
-  uint16_t w;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(address));
-  return w;
-}
-__device__ __forceinline__ float2 load_pair(uint32_t address) {  // (scale, offset)
-  uint32_t w;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(address));
-  return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+__device__ __forceinline__ float2 load_pair(const uint8_t *from) {  // (scale, offset)
+  return __half22float2(*reinterpret_cast<const __half2 *>(from));
 }
 
 __device__ __forceinline__ void bulk_copy(uint32_t to, const void *from, uint32_t bytes, uint32_t barrier) {
@@ -170,75 +195,89 @@ __device__ __forceinline__ bool wait(uint32_t barrier, uint32_t parity, volatile
 
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
 
+// a / b for a >= 0, b > 0.  Out of line: the 64-bit division is some hundred
+// instructions that hardly any call needs.
+__device__ __noinline__ int64_t divide_long(int64_t a, int64_t b) { return a / b; }
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return divide_long(a, b);
+}
+
 // A stretch of one unit's tiles: a unit is a slot and a block of its query rows.
 struct Segment {
-  int32_t slot;
-  int32_t length, tokens, first_token;  // of the slot, its sequence
+  int64_t unit_start;                   // where the unit begins among all units' tiles
+  int32_t unit_tiles;
+  int32_t slot, sequence;
+  int32_t tokens, first_token;          // of the sequence
   int32_t row0;                         // first query row (token * groups + head in group) of the unit
+  int32_t length;                       // of the slot
   int32_t tile0, tile1;                 // tiles of the stretch, those beyond every query's rows left out
   int32_t seen_max, seen_min;           // rows seen by the unit's last and first query
   bool starts, ends;                    // the stretch holds the unit's first / last tile
-  int64_t unit_start;
-  int32_t unit_tiles;
 };
 
-// The blocks' shares of all units' tiles, laid end to end.
+static_assert(sizeof(Segment) <= 64, "the layout keeps 64 bytes for a segment");
+
+// What a slot asks for: tiles per unit (at least one, so that a query without
+// a visible row gets its zeros), and units.
+template <int ROWS>
+__device__ __forceinline__ void slot_work(const AttentionParam &p, int32_t slot, Segment &s, int32_t &units) {
+  s.slot = slot;
+  s.sequence = p.by_heads(slot);
+  s.first_token = min(max(p.token_starts[s.sequence], 0), p.tokens);
+  s.tokens = max(min(p.token_starts[s.sequence + 1], p.tokens) - s.first_token, 0);
+  s.length = min(max(p.lengths[slot], 0), p.capacity);
+  s.unit_tiles = max((s.length + kTile - 1) / kTile, 1);
+  units = (s.tokens * p.groups + ROWS - 1) / ROWS;
+}
+
+__device__ __forceinline__ int32_t rows_seen(const AttentionParam &p, const Segment &s, int32_t row) {
+  return p.causal ? max(s.length - s.tokens + p.by_groups(row) + 1, 0) : s.length;
+}
+
+// Walks a block's share of all units' tiles, laid end to end with every unit
+// rounded up to a multiple of `round` tiles.
 template <int ROWS>
 struct Walk {
-  const AttentionParam &p;
   int64_t position, end;
   int64_t slot_start;
-  int32_t slot;
+  int32_t slot, round;
 
-  __device__ __forceinline__ static int32_t rows_held(const AttentionParam &p, int32_t slot) {
-    return min(max(p.lengths[slot], 0), p.capacity);
-  }
-  // A sequence's first token and its tokens, within those that there are.
-  __device__ __forceinline__ static int2 tokens_of(const AttentionParam &p, int32_t sequence) {
-    const int32_t first = min(max(p.token_starts[sequence], 0), p.tokens);
-    return make_int2(first, max(min(p.token_starts[sequence + 1], p.tokens) - first, 0));
-  }
-  __device__ __forceinline__ static int64_t cost(const AttentionParam &p, int32_t slot) {
-    const int64_t tokens = tokens_of(p, slot / p.heads).y;
-    const int64_t blocks = (tokens * p.groups + ROWS - 1) / ROWS;
-    return blocks * max((rows_held(p, slot) + kTile - 1) / kTile, 1);
-  }
-
-  __device__ __forceinline__ bool next(Segment &s) {
+  __device__ __forceinline__ bool next(const AttentionParam &p, Segment &s) {
     if (position >= end) return false;
-    int64_t whole = cost(p, slot);
-    while (position >= slot_start + whole) {
-      slot_start += whole;
-      if (++slot >= p.slots) return false;
-      whole = cost(p, slot);
+    int64_t span;
+    for (;; ++slot) {
+      if (slot >= p.slots) return false;
+      int32_t units;
+      slot_work<ROWS>(p, slot, s, units);
+      span = round == 1 ? s.unit_tiles : static_cast<int64_t>((s.unit_tiles + round - 1) / round) * round;
+      if (position < slot_start + span * units) break;
+      slot_start += span * units;
     }
-    const int2 tokens = tokens_of(p, slot / p.heads);
-    s.slot = slot;
-    s.length = rows_held(p, slot);
-    s.first_token = tokens.x;
-    s.tokens = tokens.y;
-    s.unit_tiles = max((s.length + kTile - 1) / kTile, 1);
-    const int64_t offset = position - slot_start;
-    const int64_t block = offset / s.unit_tiles;
-    s.tile0 = static_cast<int32_t>(offset - block * s.unit_tiles);
-    s.unit_start = slot_start + block * s.unit_tiles;
-    const int64_t stop = lmin(end, s.unit_start + s.unit_tiles);
-    s.tile1 = s.tile0 + static_cast<int32_t>(stop - position);
+    const int64_t unit = divide(position - slot_start, span);
+    s.unit_start = slot_start + unit * span;
+    s.tile0 = static_cast<int32_t>(position - s.unit_start);
+    const int64_t stop = lmin(end, s.unit_start + span);
+    s.tile1 = min(static_cast<int32_t>(stop - s.unit_start), s.unit_tiles);
     s.starts = s.tile0 == 0;
     s.ends = s.tile1 == s.unit_tiles;
     position = stop;
-    s.row0 = static_cast<int32_t>(block * ROWS);
-    const int32_t last_row = min(s.row0 + ROWS, s.tokens * p.groups) - 1;
-    s.seen_min = seen(p, s, s.row0);
-    s.seen_max = seen(p, s, last_row);
+    s.row0 = static_cast<int32_t>(unit * ROWS);
+    s.seen_min = rows_seen(p, s, s.row0);
+    s.seen_max = rows_seen(p, s, min(s.row0 + ROWS, s.tokens * p.groups) - 1);
     s.tile1 = min(s.tile1, (s.seen_max + kTile - 1) / kTile);
     return true;
   }
-  __device__ __forceinline__ static int32_t seen(const AttentionParam &p, const Segment &s, int32_t row) {
-    if (!p.causal) return s.length;
-    const int64_t rows = static_cast<int64_t>(s.length) - s.tokens + row / p.groups + 1;
-    return static_cast<int32_t>(rows < 0 ? 0 : rows);
-  }
+};
+
+// A block's shared words beside the ring.
+struct Control {
+  int64_t sums[2][kWarps + 1];
+  int64_t slot_start;
+  int32_t slot;
+  int32_t abort;
+  int32_t arrived[2];
+  Segment pending[2];
 };
 
 template <typename T, int D, int GROUP, int NT>
@@ -248,14 +287,25 @@ struct Consumer {
   static constexpr int kNG = L::kGroups;
   using P = std::conditional_t<GROUP == 0, T, __half>;  // the weights' type, as the matrix instruction wants V's
 
+  // Weights are exp2(s - top): top is the running maximum less kHead, so that
+  // small weights stay in f16's normal range (a weight is rounded to 11 bits
+  // down to 2^-26 of the largest; with kHead = 0 it would be 2^-14, which cost
+  // a third of a bf16 output's precision over 34,768 rows).  For 4-bit rows the
+  // operand is weight * scale: 2^12 * 8 = 2^15 while a value's scale is at most
+  // 8; `lift` (0 until then) raises top where a larger one is met.
+  static constexpr float kHead = GROUP == 0 ? (sizeof(P) == 2 && std::is_same<P, __half>::value ? 14.0f : 0.0f) : 12.0f;
+  static constexpr uint32_t kPlainScale = 0x4800;  // 8.0 in f16
+
   float out[kOut][NT][4];
   float top[NT][2], sum[NT][2];
-  float offset_sum[NT][kNG][2], scaled_sum[NT][kNG][4];
-  uint32_t query[NT <= 2 ? NT : 1][D / 16][2];
+  float lift;
+  float offset_sum[NT][kNG][2];
+  float scaled_sum[NT][(kNG + 1) / 2][4];  // of group gi: elements 2 (gi mod 2) and after
   float factor[NT][2];
   int32_t seen[NT][2];
 
   __device__ __forceinline__ void clear() {
+    lift = 0.0f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -263,7 +313,7 @@ struct Consumer {
 #pragma unroll
         for (int m = 0; m < kOut; ++m) out[m][nt][i] = 0.0f;
 #pragma unroll
-        for (int g = 0; g < kNG; ++g) scaled_sum[nt][g][i] = 0.0f;
+        for (int g = 0; g < (kNG + 1) / 2; ++g) scaled_sum[nt][g][i] = 0.0f;
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -275,97 +325,133 @@ struct Consumer {
     }
   }
 
-  __device__ __forceinline__ void query_fragment(uint32_t query_at, int nt, int ks, int lane, uint32_t *b) const {
-    if constexpr (NT <= 2) {
-      b[0] = query[nt][ks][0];
-      b[1] = query[nt][ks][1];
-    } else {
-      load_words<2>(query_at + ((nt * (D / 16) + ks) * 32 + lane) * 8, b);
-    }
+  // B operands of k-steps 2 pair and 2 pair + 1.
+  __device__ __forceinline__ static void query_fragments(const uint8_t *query_at, int nt, int pair, int lane,
+                                                         uint32_t *b) {
+    load_words<4>(query_at + ((nt * (D / 32) + pair) * 32 + lane) * 16, b);
   }
 
-  // Scores of 16 rows (first row: row0 of the tile) against the block's query
-  // rows: s[nt][0..1] of row pi(g), s[nt][2..3] of row 8 + pi(g).
-  __device__ __forceinline__ void scores(uint32_t stage, uint32_t query_at, const float *group_sums, int half, int lane,
-                                         float (*s)[4]) {
+  // Raises `lift` where a value's scale in this tile asks for it.  Rows that
+  // are not visible may hold anything; they can only raise it too far.
+  __device__ __forceinline__ void check_scales(const uint8_t *stage, int lane) {
+    uint32_t w[kNG], largest = 0;
+    load_words<kNG>(stage + 2 * L::kCodes + L::kScales + lane * L::kScaleBytes, w);
+#pragma unroll
+    for (int gi = 0; gi < kNG; ++gi) largest = max(largest, w[gi] & 0xffffu);
+    if (!__any_sync(0xffffffffu, largest > kPlainScale)) return;
+    uint32_t exponent = 0;  // f16's, of the largest finite scale
+#pragma unroll
+    for (int gi = 0; gi < kNG; ++gi)
+      if ((w[gi] & 0xffffu) < 0x7c00u) exponent = max(exponent, (w[gi] & 0xffffu) >> 10);
+    exponent = __reduce_max_sync(0xffffffffu, exponent);
+    lift = fmaxf(lift, static_cast<float>(static_cast<int>(exponent) - 17));  // scale < 2^(exponent - 14)
+  }
+
+  // Scores of the tile's rows against the block's query rows, both halves of 16
+  // rows side by side: s[half][nt][0..1] of row pi(g), [2..3] of row 8 + pi(g).
+  // pi(g) = g ^ (g >> 1 & 1), so that keys (rows by g) and values (rows by t)
+  // both spread over the banks; 16-bit rows are swizzled and take pi(g) = g.
+  __device__ __forceinline__ void scores(const uint8_t *stage, const uint8_t *query_at, const float *group_sums, int lane,
+                                         float (*s)[NT][4]) {
     const int g = lane >> 2, t = lane & 3;
-    const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if constexpr (GROUP == 0) {
-      const int row = half * 16 + (lane & 15);
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        uint32_t a[4], b[2];
-        const uint32_t address = stage + (ks >> 2) * (kTile * 128) + row * 128 +
-                                 (((2 * (ks & 3) + (lane >> 4)) ^ (row & 7)) << 4);
-        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                     : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
-                     : "r"(address));
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          query_fragment(query_at, nt, ks, lane, b);
-          mma(static_cast<const P *>(nullptr), s[nt], a, b[0], b[1], ks == 0 ? zero : s[nt]);
-        }
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[nt][i] *= factor[nt][i & 1];
-    } else {
-      const int row = half * 16 + (g ^ ((g >> 1) & 1));
-#pragma unroll
-      for (int gi = 0; gi < kNG; ++gi) {
-        uint32_t w[2][GROUP / 32];
-        const uint32_t address = stage + row * L::kRowBytes + gi * (GROUP / 2) + t * (GROUP / 8);
-        load_words<GROUP / 32>(address, w[0]);
-        load_words<GROUP / 32>(address + 8 * L::kRowBytes, w[1]);
-        float acc[NT][4], q[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const float2 pair = *reinterpret_cast<const float2 *>(group_sums + gi * L::kRows + nt * 8 + 2 * t);
-          q[nt][0] = pair.x;
-          q[nt][1] = pair.y;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[nt][i] = -8.0f * q[nt][i & 1];
-        }
-#pragma unroll
-        for (int j = 0; j < GROUP / 32; ++j) {
-          const uint32_t x0 = w[0][j], x1 = w[1][j], y0 = x0 >> 8, y1 = x1 >> 8;
-          const uint32_t low[4] = {x0 & 0x000f000fu, x1 & 0x000f000fu, y0 & 0x000f000fu, y1 & 0x000f000fu};
-          const uint32_t high[4] = {x0 & 0x00f000f0u, x1 & 0x00f000f0u, y0 & 0x00f000f0u, y1 & 0x00f000f0u};
-          const int ks = gi * (GROUP / 16) + 2 * j;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            uint32_t b[2];
-            query_fragment(query_at, nt, ks, lane, b);
-            mma(static_cast<const P *>(nullptr), acc[nt], low, b[0], b[1], acc[nt]);
-            query_fragment(query_at, nt, ks + 1, lane, b);
-            mma(static_cast<const P *>(nullptr), acc[nt], high, b[0], b[1], acc[nt]);
-          }
-        }
-        const uint32_t scales = stage + L::kCodes + (row * kNG + gi) * 4;
-        const float2 k0 = load_pair(scales), k1 = load_pair(scales + 8 * kNG * 4);
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 k = i < 2 ? k0 : k1;
-            const float x = gi == 0 ? k.y * q[nt][i & 1] : fmaf(k.y, q[nt][i & 1], s[nt][i]);
-            s[nt][i] = fmaf(k.x, acc[nt][i], x);
+          for (int i = 0; i < 4; ++i) s[half][nt][i] = 0.0f;
+#pragma unroll
+      for (int pair = 0; pair < D / 32; ++pair) {
+        uint32_t a[2][2][4];
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int row = half * 16 + (lane & 15), ks = 2 * pair + k;
+            const uint32_t address = shared_address(stage) + (ks >> 2) * (kTile * 128) + row * 128 +
+                                     (((2 * (ks & 3) + (lane >> 4)) ^ (row & 7)) << 4);
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(a[half][k][0]), "=r"(a[half][k][1]), "=r"(a[half][k][2]), "=r"(a[half][k][3])
+                         : "r"(address)
+                         : "memory");
           }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          uint32_t b[4];
+          query_fragments(query_at, nt, pair, lane, b);
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+              mma(static_cast<const P *>(nullptr), s[half][nt], a[half][k], b[2 * k], b[2 * k + 1], s[half][nt]);
+        }
       }
+    } else {
+      const int row = g ^ ((g >> 1) & 1);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int gi = 0; gi < kNG; ++gi) {
+        uint32_t w[4][GROUP / 32];
+        const uint8_t *address = stage + row * L::kRowBytes + gi * (GROUP / 2) + t * (GROUP / 8);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[nt][i] *= factor[nt][i & 1];
+        for (int r = 0; r < 4; ++r) load_words<GROUP / 32>(address + 8 * r * L::kRowBytes, w[r]);
+        float acc[2][NT][4], q[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float4 sums = *reinterpret_cast<const float4 *>(group_sums + 2 * (gi * L::kRows + nt * 8 + 2 * t));
+          q[nt][0] = sums.x;
+          q[nt][1] = sums.z;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[0][nt][i] = acc[1][nt][i] = i & 1 ? sums.w : sums.y;
+        }
+#pragma unroll
+        for (int j = 0; j < GROUP / 32; ++j) {
+          uint32_t low[2][4], high[2][4];
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const uint32_t x = w[2 * half + r][j], y = x >> 8;
+              low[half][r] = x & 0x000f000fu;
+              low[half][r + 2] = y & 0x000f000fu;
+              high[half][r] = x & 0x00f000f0u;
+              high[half][r + 2] = y & 0x00f000f0u;
+            }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            uint32_t b[4];
+            query_fragments(query_at, nt, gi * (GROUP / 32) + j, lane, b);
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+              mma(static_cast<const P *>(nullptr), acc[half][nt], low[half], b[0], b[1], acc[half][nt]);
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+              mma(static_cast<const P *>(nullptr), acc[half][nt], high[half], b[2], b[3], acc[half][nt]);
+          }
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint8_t *scales = stage + L::kCodes + ((half * 16 + row) * kNG + gi) * 4;
+          const float2 k0 = load_pair(scales), k1 = load_pair(scales + 8 * kNG * 4);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 k = i < 2 ? k0 : k1;
+              const float x = gi == 0 ? k.y * q[nt][i & 1] : fmaf(k.y, q[nt][i & 1], s[half][nt][i]);
+              s[half][nt][i] = fmaf(k.x, acc[half][nt][i], x);
+            }
+        }
+      }
     }
   }
 
   // Adds 16 rows' weighted values to the output.  With MASKED, rows that a
   // query does not see add nothing, whatever their scales hold.
   template <bool MASKED>
-  __device__ __forceinline__ void values(uint32_t stage, int half, int lane, const float (*w)[4], int32_t first_row) {
+  __device__ __forceinline__ void values(const uint8_t *stage, int half, int lane, const float (*w)[4], int32_t first_row) {
     const int g = lane >> 2, t = lane & 3;
-    const uint32_t values_at = stage + L::kCodes + L::kScales;
+    const uint8_t *values_at = stage + L::kCodes + L::kScales;
     if constexpr (GROUP == 0) {
       uint32_t b[NT][2];
 #pragma unroll
@@ -377,11 +463,12 @@ struct Consumer {
 #pragma unroll
       for (int m = 0; m < kOut; ++m) {
         uint32_t a[4];
-        const uint32_t address = values_at + (m >> 2) * (kTile * 128) + row * 128 +
+        const uint32_t address = shared_address(values_at) + (m >> 2) * (kTile * 128) + row * 128 +
                                  (((2 * (m & 3) + ((lane >> 3) & 1)) ^ (row & 7)) << 4);
         asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                      : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
-                     : "r"(address));
+                     : "r"(address)
+                     : "memory");
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
           mma(static_cast<const P *>(nullptr), out[m][nt], a, b[nt][0], b[nt][1], out[m][nt]);
@@ -392,35 +479,36 @@ struct Consumer {
       const int other = half * 16 + 2 * t + (1 ^ (t & 1));   // pi(2t), pi(2t + 1), and 8 later
 #pragma unroll
       for (int gi = 0; gi < kNG; ++gi) {
-        const uint32_t scales = values_at + L::kCodes + (row * kNG + gi) * 4;
+        const uint8_t *scales = values_at + L::kCodes + (row * kNG + gi) * 4;
         const float2 v0 = load_pair(scales), v1 = load_pair(scales + 8 * kNG * 4);
         uint32_t b[NT][2];
-        const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+        // Ones in the upper or the lower eight rows: two groups share an accumulator.
+        const uint32_t up = gi & 1 ? 0u : 0x3c003c00u, down = gi & 1 ? 0x3c003c00u : 0u;
+        const uint32_t ones[4] = {up, down, up, down};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float scaled[4], shift[4];
+          float scaled[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float2 v = i < 2 ? v0 : v1;
             const bool none = MASKED && first_row + row + (i < 2 ? 0 : 8) >= seen[nt][i & 1];
             scaled[i] = none ? 0.0f : w[nt][i] * v.x;
-            shift[i] = none ? 0.0f : w[nt][i] * v.y;
+            float &sum_of = offset_sum[nt][gi][i & 1];
+            sum_of = none ? sum_of : fmaf(w[nt][i], v.y, sum_of);
           }
           b[nt][0] = transpose8(pack(static_cast<const P *>(nullptr), scaled[0], scaled[1]));
           b[nt][1] = transpose8(pack(static_cast<const P *>(nullptr), scaled[2], scaled[3]));
-          offset_sum[nt][gi][0] += shift[0] + shift[2];
-          offset_sum[nt][gi][1] += shift[1] + shift[3];
-          mma(static_cast<const P *>(nullptr), scaled_sum[nt][gi], ones, b[nt][0], b[nt][1], scaled_sum[nt][gi]);
+          mma(static_cast<const P *>(nullptr), scaled_sum[nt][gi / 2], ones, b[nt][0], b[nt][1], scaled_sum[nt][gi / 2]);
         }
-        const uint32_t at = values_at + gi * (GROUP / 2) + g * (GROUP / 16);
+        const uint8_t *at = values_at + gi * (GROUP / 2) + g * (GROUP / 16);
         constexpr int kWords = GROUP == 128 ? 2 : 1;
         constexpr int kBytes = GROUP / 16 / kWords;  // of a word that are used
         uint32_t x[4][kWords];
-        const uint32_t rows[4] = {at + token * L::kRowBytes, at + other * L::kRowBytes,
+        const uint8_t *rows[4] = {at + token * L::kRowBytes, at + other * L::kRowBytes,
                                   at + (token + 8) * L::kRowBytes, at + (other + 8) * L::kRowBytes};
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          if constexpr (GROUP == 32) x[r][0] = load_short(rows[r]);
+          if constexpr (GROUP == 32) x[r][0] = *reinterpret_cast<const uint16_t *>(rows[r]);
           else load_words<kWords>(rows[r], x[r]);
         }
 #pragma unroll
@@ -441,11 +529,12 @@ struct Consumer {
   }
 
   template <bool MASKED>
-  __device__ __forceinline__ void tile(uint32_t stage, uint32_t query_at, const float *group_sums, int lane,
+  __device__ __forceinline__ void tile(uint8_t *stage, const uint8_t *query_at, const float *group_sums, int lane,
                                        int32_t first_row, int32_t seen_max) {
     float s[2][NT][4];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) scores(stage, query_at, group_sums, half, lane, s[half]);
+    const float lifted = lift;
+    if constexpr (GROUP != 0) check_scales(stage, lane);
+    scores(stage, query_at, group_sums, lane, s);
     if constexpr (MASKED) {
       const int g = lane >> 2;
       const int row = first_row + (GROUP == 0 ? g : g ^ ((g >> 1) & 1));
@@ -457,18 +546,18 @@ struct Consumer {
           for (int i = 0; i < 4; ++i)
             if (row + half * 16 + (i < 2 ? 0 : 8) >= seen[nt][i & 1]) s[half][nt][i] = -INFINITY;
     }
-    bool grows = false;
+    bool grows = lift != lifted;
     float best[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         // max_nan: a NaN score makes the maximum, and with it the result, NaN.
-        float m = max_nan(max_nan(s[0][nt][i], s[0][nt][i + 2]), max_nan(s[1][nt][i], s[1][nt][i + 2]));
+        float m = max_nan(max_nan(s[0][nt][i], s[0][nt][i + 2], s[1][nt][i]), s[1][nt][i + 2]);
         m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 4));
         m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 8));
         m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 16));
-        best[nt][i] = max_nan(m, top[nt][i]);
+        best[nt][i] = max_nan(fmaf(m, factor[nt][i], lift - kHead), top[nt][i] + (lift - lifted));
         grows |= best[nt][i] != top[nt][i];
       }
     if (__any_sync(0xffffffffu, grows)) {
@@ -482,8 +571,7 @@ struct Consumer {
 #pragma unroll
           for (int g = 0; g < kNG; ++g) {
             offset_sum[nt][g][i] *= keep;
-            scaled_sum[nt][g][i] *= keep;
-            scaled_sum[nt][g][i + 2] *= keep;
+            scaled_sum[nt][g / 2][i + 2 * (g & 1)] *= keep;
           }
 #pragma unroll
           for (int m = 0; m < kOut; ++m) {
@@ -499,21 +587,18 @@ struct Consumer {
         const float m = top[nt][i] == -INFINITY ? 0.0f : top[nt][i];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          s[half][nt][i] = exp2_fast(s[half][nt][i] - m);
-          s[half][nt][i + 2] = exp2_fast(s[half][nt][i + 2] - m);
+          s[half][nt][i] = exp2_fast(fmaf(s[half][nt][i], factor[nt][i], -m));
+          s[half][nt][i + 2] = exp2_fast(fmaf(s[half][nt][i + 2], factor[nt][i], -m));
         }
         sum[nt][i] += (s[0][nt][i] + s[0][nt][i + 2]) + (s[1][nt][i] + s[1][nt][i + 2]);
       }
     if constexpr (MASKED && GROUP == 0) {
       // What lies beyond every query's rows may be NaN, and 0 NaN is NaN.
-      const uint32_t values_at = stage + L::kCodes;
       if (first_row + lane >= seen_max)
 #pragma unroll
         for (int c = 0; c < D / 8; ++c)
-          asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(values_at + (c >> 3) * (kTile * 128) + lane * 128 +
-                                                                    (c & 7) * 16),
-                       "r"(0)
-                       : "memory");
+          *reinterpret_cast<uint4 *>(stage + L::kCodes + (c >> 3) * (kTile * 128) + lane * 128 + (c & 7) * 16) =
+              make_uint4(0, 0, 0, 0);
       __syncwarp();
     }
 #pragma unroll
@@ -521,37 +606,62 @@ struct Consumer {
   }
 };
 
+// Adds a part's (maximum, sum) to another's.
+__device__ __forceinline__ void add_part(float &best, float &sum, float m, float l) {
+  const float next = max_nan(best, m);
+  sum = (best == -INFINITY ? 0.0f : sum * exp2_fast(best - next)) + (m == -INFINITY ? 0.0f : l * exp2_fast(m - next));
+  best = next;
+}
+
+// lse of weights exp2(s - top) that add up to sum.
+__device__ __noinline__ float natural(float top, float sum) {
+  return sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945f;
+}
+
+// The output row of a unit's query row.
+__device__ __forceinline__ int64_t out_row(const AttentionParam &p, const Segment &s, int32_t query_row) {
+  const int32_t token = p.by_groups(query_row), head = s.slot - s.sequence * p.heads;
+  return (static_cast<int64_t>(s.first_token + token) * p.heads + head) * p.groups + (query_row - token * p.groups);
+}
+
 template <typename T, int D, int GROUP, int NT>
 __global__ __launch_bounds__(kThreads, (Layout<T, D, GROUP, NT>::kBlocksPerSm))
-void attention_kernel(const AttentionParam p, const __grid_constant__ CUtensorMap key_map,
+void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_constant__ CUtensorMap key_map,
                       const __grid_constant__ CUtensorMap value_map) {
   using L = Layout<T, D, GROUP, NT>;
-  extern __shared__ uint8_t shared_raw[];
-  uint8_t *shared = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(shared_raw) + 1023) & ~uintptr_t{1023});
-  const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(shared));
+  static_assert(sizeof(Control) <= L::kControl, "Control has grown");
+  extern __shared__ __align__(1024) uint8_t shared[];
+  const uint32_t base = shared_address(shared);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t full = base + L::kBarriersAt, empty = full + L::kStages * 8;
-  int64_t *walk_start = reinterpret_cast<int64_t *>(shared + L::kBarriersAt + 2 * L::kStages * 8);  // slot_start, total
-  int32_t *walk_slot = reinterpret_cast<int32_t *>(walk_start + 2);
-  volatile int *abort = walk_slot + 1;
-  int *arrived = const_cast<int *>(walk_slot) + 2;
+  Control &control = *reinterpret_cast<Control *>(shared + L::kBarriersAt + 2 * L::kStages * 8);
+  volatile int *abort = &control.abort;
+  if (base & 1023) {  // the 128-byte swizzle goes by address bits
+    if (threadIdx.x == 0) atomicOr(p.flag, kFlagTimeout);
+    return;
+  }
 
-  // This block's stretch: a scan of every slot's tiles.
-  __shared__ int64_t warp_sums[kWarps + 1];
+  // All slots' tiles and units, and from them the blocks' share.
   const int32_t each = (p.slots + kThreads - 1) / kThreads;
   const int32_t mine0 = min(static_cast<int32_t>(threadIdx.x) * each, p.slots), mine1 = min(mine0 + each, p.slots);
-  int64_t mine = 0;
-  for (int32_t s = mine0; s < mine1; ++s) {
-    mine += Walk<L::kRows>::cost(p, s);
-    if (blockIdx.x == 0 && p.lengths[s] > p.capacity) atomicOr(p.flag, kFlagRow);
+  int64_t tiles_sum = 0, units_sum = 0;
+  Segment s;
+  int32_t units = 0;
+  for (int32_t i = mine0; i < mine1; ++i) {
+    slot_work<L::kRows>(p, i, s, units);
+    units_sum += units;
+    tiles_sum += static_cast<int64_t>(units) * s.unit_tiles;
+    if (blockIdx.x == 0 && p.lengths[i] > p.capacity) atomicOr(p.flag, kFlagRow);
   }
-  int64_t before = mine;
 #pragma unroll
-  for (int step = 1; step < 32; step <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, before, step);
-    if (lane >= step) before += x;
+  for (int step = 16; step > 0; step >>= 1) {
+    tiles_sum += __shfl_xor_sync(0xffffffffu, tiles_sum, step);
+    units_sum += __shfl_xor_sync(0xffffffffu, units_sum, step);
   }
-  if (lane == 31) warp_sums[warp] = before;
+  if (lane == 0) {
+    control.sums[0][warp] = tiles_sum;
+    control.sums[1][warp] = units_sum;
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kStages; ++i) {
       tc::init_barrier(full + i * 8, 1);
@@ -561,178 +671,205 @@ void attention_kernel(const AttentionParam p, const __grid_constant__ CUtensorMa
     *abort = 0;
   }
   __syncthreads();
+  tiles_sum = units_sum = 0;
+#pragma unroll
+  for (int w = 0; w <= kWarps; ++w) {
+    tiles_sum += control.sums[0][w];
+    units_sum += control.sums[1][w];
+  }
+  // With few units a block takes a piece of one unit (a unit rounded up to
+  // whole pieces): sum ceil(tiles / share) <= tiles_sum / share + units <=
+  // grid.  A second unit costs a block its start and its end once more, some
+  // 4 us; rounding costs the blocks units / grid of their time.  So with many
+  // units the shares are equal and cross the units' ends.
+  const bool pieces_apart = units_sum * 4 <= gridDim.x;
+  const int64_t blocks = pieces_apart ? gridDim.x - units_sum : gridDim.x;
+  const int64_t share = lmax(divide(tiles_sum + blocks - 1, blocks), kMinTiles);
+  Walk<L::kRows> walk;
+  walk.round = pieces_apart ? static_cast<int32_t>(share) : 1;
+  int64_t mine = 0;
+  for (int32_t i = mine0; i < mine1; ++i) {
+    if (mine1 - mine0 > 1) slot_work<L::kRows>(p, i, s, units);
+    mine += units * (pieces_apart ? static_cast<int64_t>((s.unit_tiles + walk.round - 1) / walk.round) * walk.round
+                                  : s.unit_tiles);
+  }
+  int64_t before = mine;
+#pragma unroll
+  for (int step = 1; step < 32; step <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, before, step);
+    if (lane >= step) before += x;
+  }
+  __syncthreads();  // the sums have been read
+  if (lane == 31) control.sums[0][warp] = before;
+  __syncthreads();
   int64_t total = 0;
 #pragma unroll
   for (int w = 0; w <= kWarps; ++w) {
-    if (w < warp) before += warp_sums[w];
-    total += warp_sums[w];
+    if (w < warp) before += control.sums[0][w];
+    total += control.sums[0][w];
   }
   before -= mine;
-  const int64_t share = lmax((total + gridDim.x - 1) / gridDim.x, kMinTiles);
-  const int64_t start = share * blockIdx.x;
-  if (start >= total) return;
-  if (start >= before && start < before + mine) {
-    int32_t s = mine0;
-    for (int64_t c; start >= before + (c = Walk<L::kRows>::cost(p, s)); ++s) before += c;
-    walk_start[0] = before;
-    *walk_slot = s;
+  walk.position = share * blockIdx.x;
+  if (walk.position >= total) return;
+  walk.end = lmin(walk.position + share, total);
+  if (walk.position >= before && walk.position < before + mine) {
+    control.slot_start = before;
+    control.slot = mine0;
   }
   __syncthreads();
-  Walk<L::kRows> walk{p, start, lmin(start + share, total), walk_start[0], *walk_slot};
-  Segment s;
+  walk.slot_start = control.slot_start;
+  walk.slot = control.slot;
 
-  if (warp == kWarps) {
-    // The feeding warp: every tile of the stretch in order, through the ring.
-    int64_t count = 0;
-    while (walk.next(s)) {
-      const int32_t *entries = p.table + static_cast<int64_t>(s.slot) * p.table_stride;
-      for (int32_t first = s.tile0; first < s.tile1; first += 32) {
-        // Lane i looks up the page(s) of tile first + i.
-        const int32_t ahead = first + lane;
-        int32_t page[2] = {0, 0};
-        constexpr int kParts = 2;
-        const int parts = p.pages.page_size == 16 ? kParts : 1;
-        if (ahead < s.tile1)
-          for (int part = 0; part < parts; ++part) {
-            const int32_t row = ahead * kTile + part * 16;
-            if (row >= s.seen_max) break;
-            page[part] = entries[row >> p.pages.page_shift];
-            if (page[part] < 0 || page[part] >= p.pages.pages) {
-              page[part] = 0;
-              atomicOr(p.flag, kFlagRow);
-            }
-          }
-        const int32_t last = min(first + 32, s.tile1);
-        for (int32_t tile = first; tile < last; ++tile, ++count) {
-          const int32_t page0 = __shfl_sync(0xffffffffu, page[0], tile - first);
-          const int32_t page1 = __shfl_sync(0xffffffffu, page[1], tile - first);
-          const int stage = static_cast<int>(count % L::kStages);
-          const uint32_t phase = static_cast<uint32_t>(count / L::kStages) & 1;
-          const uint32_t at = base + stage * L::kStage, barrier = full + stage * 8;
-          if (count >= L::kStages && !wait(empty + stage * 8, phase ^ 1, abort)) {
-            if (lane == 0) atomicOr(p.flag, kFlagTimeout);
-            goto drained;
-          }
-          const int32_t row = tile * kTile;
-          const int copies = parts == 1 || row + 16 >= s.seen_max ? 1 : 2;  // pages that the tile's rows lie in
-          const int rows = parts == 1 ? kTile : 16;
-          if (lane == 0) tc::expect_bytes(barrier, copies * rows * (L::kStage / kTile));
-          __syncwarp();
-          if constexpr (GROUP == 0) {
-            constexpr int kBoxes = D / 64;  // 64 channels wide, per tensor and page
-            if (lane < copies * 2 * kBoxes) {
-              const int part = lane / (2 * kBoxes), side = (lane / kBoxes) & 1, box = lane % kBoxes;
-              const int64_t y = static_cast<int64_t>(part ? page1 : page0) * p.pages.page_size +
-                                (row & (p.pages.page_size - 1));
-              tc::tma_box(at + side * L::kCodes + box * (kTile * 128) + part * 16 * 128, side ? &value_map : &key_map,
-                          box * 64, static_cast<int>(y), barrier);
-            }
-          } else {
-            if (lane < copies * 4) {
-              const int part = lane >> 2, side = (lane >> 1) & 1;
-              const bool scales = lane & 1;
-              const int64_t y = static_cast<int64_t>(part ? page1 : page0) * p.pages.page_size +
-                                (row & (p.pages.page_size - 1));
-              const uint32_t to = at + side * (L::kCodes + L::kScales);
-              if (scales) {
-                const uint8_t *from = reinterpret_cast<const uint8_t *>(side ? p.pages.value_scales : p.pages.key_scales);
-                bulk_copy(to + L::kCodes + part * 16 * L::kScaleBytes, from + y * L::kScaleBytes, rows * L::kScaleBytes,
-                          barrier);
-              } else {
-                const uint8_t *from = side ? p.pages.values : p.pages.keys;
-                bulk_copy(to + part * 16 * L::kRowBytes, from + y * L::kRowBytes, rows * L::kRowBytes, barrier);
-              }
-            }
-          }
-        }
-      }
-    }
-    return;
-  drained:
-    // Given up: leave only after the copies in flight have landed.
-    for (int64_t c = count > L::kStages ? count - L::kStages : 0; c < count; ++c)
-      tc::wait_phase(full + static_cast<int>(c % L::kStages) * 8, static_cast<uint32_t>(c / L::kStages) & 1, nullptr);
-    return;
-  }
-
+  // The feeding warp's place in the ring, or a consumer's next tile of it.
+  int stage = warp == kWarps ? 0 : warp;
+  uint32_t phase = 0;
+  int64_t fed = 0;
+  bool failed = false;
   Consumer<T, D, GROUP, NT> c;
   float *group_sums = reinterpret_cast<float *>(shared + L::kSumsAt);
   float *factors = reinterpret_cast<float *>(shared + L::kFactorAt);
   float *stat_top = reinterpret_cast<float *>(shared + L::kStatsAt), *stat_sum = stat_top + kWarps * L::kRows;
   float *scratch = reinterpret_cast<float *>(shared + L::kScratchAt);
-  const uint32_t query_at = base + L::kQueryAt;
+  const uint8_t *query_at = shared + L::kQueryAt;
   const int g = lane >> 2, t = lane & 3;
-  int64_t done = 0;  // tiles of the stretch before this segment
-  while (walk.next(s)) {
-    const int32_t sequence = s.slot / p.heads, head = s.slot - sequence * p.heads;
-    const int32_t rows_total = s.tokens * p.groups;
-    const int64_t query_heads = static_cast<int64_t>(p.heads) * p.groups;
-    // Query fragments, one 8-row tile per warp: B operand of k-step ks holds,
-    // for query row g, the channels of the matching A registers.
-    for (int nt = warp; nt < NT; nt += kWarps) {
-      const int32_t row = s.row0 + nt * 8 + g;
-      const bool live = row < rows_total;
-      const T *from = static_cast<const T *>(p.queries) +
-                      static_cast<int64_t>(s.first_token + (live ? row / p.groups : 0)) * p.query_token +
-                      (static_cast<int64_t>(head) * p.groups + (live ? row % p.groups : 0)) * p.query_head;
-      uint2 *to = reinterpret_cast<uint2 *>(shared + L::kQueryAt) + nt * (D / 16) * 32 + lane;
-      if constexpr (GROUP == 0) {
+  // A negative scale is taken by the queries, so that the largest score is the
+  // largest product; the factor stays above zero for the sake of -inf.
+  const uint32_t turn = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
+  constexpr float kLeastFactor = 1e-37f;
+  int pieces = 0;
+  int turn_of = 0;  // the warp that the segment's first tile falls to
+
+  while (walk.next(p, s)) {
+    if (warp == kWarps) {
+      // The feeding warp: every tile of the stretch in order, through the ring.
+      const int32_t *entries = p.table + static_cast<int64_t>(s.slot) * p.table_stride;
+      for (int32_t first = s.tile0; first < s.tile1 && !failed; first += 32) {
+        // Lane i looks up the page(s) of tile first + i, and later issues its copies.
+        const int32_t row = (first + lane) * kTile;
+        const int parts = p.pages.page_size == 16 ? 2 : 1;
+        const int rows = parts == 1 ? kTile : 16;  // of a part
+        int copies = 0;                            // parts that the tile's visible rows lie in
+        int64_t y[2] = {0, 0};
+        if (first + lane < s.tile1) {
+          copies = parts == 1 || row + 16 >= s.seen_max ? 1 : 2;
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t *pair = reinterpret_cast<const uint32_t *>(from + ks * 16 + 2 * t);
-          to[ks * 32] = live ? make_uint2(pair[0], pair[4]) : make_uint2(0, 0);
+          for (int part = 0; part < 2; ++part)
+            if (part < copies) {
+              int32_t page = entries[(row + part * 16) >> p.pages.page_shift];
+              if (page < 0 || page >= p.pages.pages) {
+                page = 0;
+                atomicOr(p.flag, kFlagRow);
+              }
+              y[part] = static_cast<int64_t>(page) * p.pages.page_size + (row & (p.pages.page_size - 1));
+            }
         }
-        if (t == 0) factors[nt * 8 + g] = p.scale_log2;
-      } else {
-        // This lane's D / 4 channels: GROUP / 4 of each group.
-        float q[D / 4];
-        float largest = 0.0f;
+        const int32_t here = min(32, s.tile1 - first);
+        for (int32_t j = 0; j < here; ++j) {
+          const uint32_t at = base + stage * L::kStage, barrier = full + stage * 8;
+          bool given_up = false;
+          if (lane == j) {
+            given_up = fed >= L::kStages && !wait(empty + stage * 8, phase ^ 1, abort);
+            if (!given_up) {
+              tc::expect_bytes(barrier, copies * rows * (L::kStage / kTile));
+              for (int part = 0; part < copies; ++part) {
+                const int64_t from = y[part];
 #pragma unroll
-        for (int gi = 0; gi < L::kGroups; ++gi)
+                for (int side = 0; side < 2; ++side) {
+                  const uint32_t to = at + side * (L::kCodes + L::kScales);
+                  if constexpr (GROUP == 0) {
 #pragma unroll
-          for (int j = 0; j < GROUP / 32; ++j) {
-            float *x = q + (gi * (GROUP / 32) + j) * 8;
-            load8(from + gi * GROUP + t * (GROUP / 4) + j * 8, x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              if (!live) x[i] = 0.0f;
-              largest = fmaxf(largest, fabsf(x[i]));
+                    for (int box = 0; box < D / 64; ++box)  // 64 channels wide
+                      tc::tma_box(to + box * (kTile * 128) + part * 16 * 128, side ? &value_map : &key_map, box * 64,
+                                  static_cast<int>(from), barrier);
+                  } else {
+                    bulk_copy(to + part * 16 * L::kRowBytes, (side ? p.pages.values : p.pages.keys) + from * L::kRowBytes,
+                              rows * L::kRowBytes, barrier);
+                    bulk_copy(to + L::kCodes + part * 16 * L::kScaleBytes,
+                              (side ? p.pages.value_scales : p.pages.key_scales) + from * L::kGroups,
+                              rows * L::kScaleBytes, barrier);
+                  }
+                }
+              }
             }
           }
-        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+          // The warp stays together: a lane that ran ahead would find an older
+          // phase of its stage's barrier with the parity that it waits for.
+          if (given_up) atomicOr(p.flag, kFlagTimeout);
+          failed = __any_sync(0xffffffffu, given_up || *abort);
+          if (failed) break;
+          ++fed;
+          if (++stage == L::kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (failed) break;
+      continue;
+    }
+
+    const int32_t head = s.slot - s.sequence * p.heads;
+    const int32_t rows_total = s.tokens * p.groups;
+    // Query fragments: the B operand of a k-step holds, for query row g, the
+    // channels of the matching A registers.  D / 8 threads a row, 8 channels each.
+    constexpr int kAcross = D / 8;
+    const int column = threadIdx.x % kAcross;
+    for (int row = threadIdx.x / kAcross; row < L::kRows; row += kWarps * 32 / kAcross) {
+      const int32_t query_row = s.row0 + row;
+      const bool live = query_row < rows_total;
+      const T *from = static_cast<const T *>(p.queries) +
+                      static_cast<int64_t>(s.first_token + (live ? p.by_groups(query_row) : 0)) * p.query_token +
+                      (static_cast<int64_t>(head) * p.groups + (live ? query_row - p.by_groups(query_row) * p.groups : 0)) * p.query_head;
+      uint8_t *to = shared + L::kQueryAt + ((row >> 3) * (D / 32) * 32 + (row & 7) * 4) * 16;
+      if constexpr (GROUP == 0) {
+        // Channels 8 column ..: the low or high 8 of k-step column / 2, whose
+        // pairs go to the four lanes of the row.
+        uint4 x = live ? *reinterpret_cast<const uint4 *>(from + column * 8) : make_uint4(0, 0, 0, 0);
+        const uint32_t pairs[4] = {x.x ^ turn, x.y ^ turn, x.z ^ turn, x.w ^ turn};
+        uint32_t *words = reinterpret_cast<uint32_t *>(to + (column >> 2) * 32 * 16) + (column & 3);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) words[i * 4] = pairs[i];
+        if (column == 0) factors[row] = fmaxf(fabsf(p.scale_log2), kLeastFactor);
+      } else {
+        float x[8];
+        load8(from + column * 8, x);
+        float largest = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (!live) x[i] = 0.0f;
+          largest = fmaxf(largest, fabsf(x[i]));
+        }
+#pragma unroll
+        for (int step = 1; step < kAcross; step <<= 1)
+          largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, step));
         // A power of two brings the row's largest value into [1, 2): f16 then
         // holds bf16 values exactly down to 2^-14 of the row's largest, and the
         // rest to 2^-25 of it.
         const int exponent = static_cast<int>(__float_as_uint(largest) >> 23);
         const bool plain = exponent == 255 || largest == 0.0f;
         const int shift = plain ? 0 : (exponent == 0 ? 1 : exponent) - 127;
-        const float to_unit = __int_as_float((127 - min(shift, 126)) << 23);
+        const float to_unit = __int_as_float(((127 - min(shift, 126)) << 23) | (turn & 0x80000000u));
         const float from_unit = __int_as_float((127 + min(shift, 127)) << 23);
+        __half h[8];
+        float group_sum = 0.0f;
 #pragma unroll
-        for (int gi = 0; gi < L::kGroups; ++gi) {
-          float group_sum = 0.0f;
-#pragma unroll
-          for (int j = 0; j < GROUP / 32; ++j) {
-            __half h[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              h[i] = __float2half_rn(q[(gi * (GROUP / 32) + j) * 8 + i] * to_unit);
-              group_sum += __half2float(h[i]);
-            }
-            const __half sixteen = __float2half_rn(16.0f);
-            const int ks = gi * (GROUP / 16) + 2 * j;
-            __half2 b[4] = {__halves2half2(__hmul(h[0], sixteen), __hmul(h[4], sixteen)),
-                            __halves2half2(__hmul(h[2], sixteen), __hmul(h[6], sixteen)), __halves2half2(h[1], h[5]),
-                            __halves2half2(h[3], h[7])};
-            to[ks * 32] = *reinterpret_cast<uint2 *>(&b[0]);
-            to[(ks + 1) * 32] = *reinterpret_cast<uint2 *>(&b[2]);
-          }
-          group_sum += __shfl_xor_sync(0xffffffffu, group_sum, 1);
-          group_sum += __shfl_xor_sync(0xffffffffu, group_sum, 2);
-          if (t == 0) group_sums[gi * L::kRows + nt * 8 + g] = group_sum * 0x1p-20f;
+        for (int i = 0; i < 8; ++i) {
+          h[i] = __float2half_rn(x[i] * to_unit);
+          group_sum += __half2float(h[i]);
         }
-        if (t == 0) factors[nt * 8 + g] = p.scale_log2 * 0x1p20f * from_unit;
+        const __half sixteen = __float2half_rn(16.0f);  // nibbles in bits 0-3 stand for a sixteenth of those in 4-7
+        __align__(16) __half2 b[4] = {__halves2half2(__hmul(h[0], sixteen), __hmul(h[4], sixteen)),
+                                      __halves2half2(__hmul(h[2], sixteen), __hmul(h[6], sixteen)),
+                                      __halves2half2(h[1], h[5]), __halves2half2(h[3], h[7])};
+        const int gi = column / (GROUP / 8), within = column % (GROUP / 8);
+        const int quarter = within / (GROUP / 32), j = within % (GROUP / 32);
+        reinterpret_cast<uint4 *>(to)[(gi * (GROUP / 32) + j) * 32 + quarter] = *reinterpret_cast<uint4 *>(b);
+#pragma unroll
+        for (int step = 1; step < GROUP / 8; step <<= 1) group_sum += __shfl_xor_sync(0xffffffffu, group_sum, step);
+        group_sum *= 0x1p-20f;
+        if (within == 0)
+          reinterpret_cast<float2 *>(group_sums)[gi * L::kRows + row] = make_float2(group_sum, -8.0f * group_sum);
+        if (column == 0) factors[row] = fmaxf(fabsf(p.scale_log2) * 0x1p20f * from_unit, kLeastFactor);
       }
     }
     consumers_sync();
@@ -742,29 +879,18 @@ void attention_kernel(const AttentionParam p, const __grid_constant__ CUtensorMa
       for (int i = 0; i < 2; ++i) {
         const int32_t row = s.row0 + nt * 8 + 2 * t + i;
         c.factor[nt][i] = factors[nt * 8 + 2 * t + i];
-        c.seen[nt][i] = row < rows_total ? Walk<L::kRows>::seen(p, s, row) : s.seen_max;
+        c.seen[nt][i] = row < rows_total ? rows_seen(p, s, row) : s.seen_max;
       }
-    if constexpr (NT <= 2) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
-          load_words<2>(query_at + ((nt * (D / 16) + ks) * 32 + lane) * 8, c.query[nt][ks]);
-    }
     c.clear();
     const int32_t tiles = max(s.tile1 - s.tile0, 0);
-    // Tile number k of the whole stretch falls to warp k mod kWarps.
-    for (int32_t i = static_cast<int32_t>((warp + kWarps - done % kWarps) % kWarps); i < tiles; i += kWarps) {
-      const int64_t k = done + i;
-      const int stage = static_cast<int>(k % L::kStages);
-      const uint32_t phase = static_cast<uint32_t>(k / L::kStages) & 1;
-      if (!wait(full + stage * 8, phase, abort)) {
-        if (lane == 0) atomicOr(p.flag, kFlagTimeout);
-        continue;  // every barrier below is still met
-      }
+    // The stretch's tiles go to the warps in turn.
+    for (int32_t i = (warp - turn_of) & (kWarps - 1); i < tiles; i += kWarps) {
+      uint8_t *const at = shared + stage * L::kStage;
+      const bool landed = wait(full + stage * 8, phase, abort);
       const int32_t first_row = (s.tile0 + i) * kTile;
-      const uint32_t at = base + stage * L::kStage;
-      if (first_row + kTile > s.seen_min) {
+      if (!landed) {  // every barrier below is still met
+        if (lane == 0) atomicOr(p.flag, kFlagTimeout);
+      } else if (first_row + kTile > s.seen_min) {
         c.template tile<true>(at, query_at, group_sums, lane, first_row, s.seen_max);
         if constexpr (GROUP == 0) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       } else {
@@ -772,8 +898,13 @@ void attention_kernel(const AttentionParam p, const __grid_constant__ CUtensorMa
       }
       __syncwarp();
       if (lane == 0) tc::arrive(empty + stage * 8);
+      stage += kWarps;
+      if (stage >= L::kStages) {
+        stage -= L::kStages;
+        phase ^= 1;
+      }
     }
-    done += tiles;
+    turn_of = (turn_of + tiles) & (kWarps - 1);
 
     // Join the warps.
 #pragma unroll
@@ -793,8 +924,7 @@ void attention_kernel(const AttentionParam p, const __grid_constant__ CUtensorMa
         }
       }
     consumers_sync();
-    const bool whole = s.starts && s.ends;
-    const bool whole_unit = whole || (s.starts && s.unit_start + s.unit_tiles <= walk.end);
+    const bool whole_unit = s.starts && s.ends;
     float *partial = p.partials + (static_cast<int64_t>(blockIdx.x) * 2 + (s.starts ? 1 : 0)) * L::kRows * (D + 2);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -815,7 +945,7 @@ void attention_kernel(const AttentionParam p, const __grid_constant__ CUtensorMa
         } else {
 #pragma unroll
           for (int gi = 0; gi < L::kGroups; ++gi) {
-            const float rest = fmaf(-8.0f, c.scaled_sum[nt][gi][i], c.offset_sum[nt][gi][i]);
+            const float rest = fmaf(-8.0f, c.scaled_sum[nt][gi / 2][i + 2 * (gi & 1)], c.offset_sum[nt][gi][i]);
 #pragma unroll
             for (int k = 0; k < GROUP / 16; ++k) {
               const int m = gi * (GROUP / 16) + k;
@@ -852,10 +982,9 @@ void attention_kernel(const AttentionParam p, const __grid_constant__ CUtensorMa
       const int32_t query_row = s.row0 + nt * 8 + row;
       if (query_row < rows_total) {
         if (whole_unit) {
-          const int64_t index = static_cast<int64_t>(s.first_token + query_row / p.groups) * query_heads +
-                                static_cast<int64_t>(head) * p.groups + query_row % p.groups;
+          const int64_t index = out_row(p, s, query_row);
           const float inverse = weight_sum == 0.0f ? 0.0f : 1.0f / weight_sum;
-          T result[kEach];
+          __align__(16) T result[kEach];
 #pragma unroll
           for (int i = 0; i < kEach; ++i) result[i] = from_float<T>(value[i] * inverse);
           if constexpr (kEach == 8)
@@ -863,7 +992,7 @@ void attention_kernel(const AttentionParam p, const __grid_constant__ CUtensorMa
           else
             *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + index * D + channel) = *reinterpret_cast<uint2 *>(result);
           if (channel == 0)
-            p.lse[index] = weight_sum == 0.0f ? -INFINITY : (best + log2f(weight_sum)) * 0.693147180559945f;
+            p.lse[index] = natural(best, weight_sum);
         } else {
 #pragma unroll
           for (int i = 0; i < kEach; i += 4)
@@ -877,61 +1006,97 @@ void attention_kernel(const AttentionParam p, const __grid_constant__ CUtensorMa
       }
       consumers_sync();
     }
-    if (whole_unit) continue;
+    if (!whole_unit) {
+      if (threadIdx.x == 0) control.pending[pieces] = s;
+      ++pieces;
+    }
+  }
 
-    // The unit's blocks are first .. last; the one that arrives last joins.
-    const int64_t first = s.unit_start / share, last = (s.unit_start + s.unit_tiles - 1) / share;
-    __threadfence();
-    consumers_sync();
-    if (threadIdx.x == 0) {
-      const uint32_t before_me = atomicAdd(p.counters + first, 1u);
-      const bool joins = before_me == static_cast<uint32_t>(last - first);
-      if (joins) p.counters[first] = 0;  // as the next call expects it
-      *arrived = joins;
-    }
-    consumers_sync();
-    if (!*arrived) continue;
-    __threadfence();
-    constexpr int kEach = D / 16;
-    const int channel = (threadIdx.x & 15) * kEach;
-    for (int row = threadIdx.x >> 4; row < L::kRows && s.row0 + row < rows_total; row += 8) {
-      auto part_at = [&](int64_t block) {
-        return p.partials + (block * 2 + (block == first ? 1 : 0)) * L::kRows * (D + 2);
-      };
-      float best = -INFINITY;
-      for (int64_t b = first; b <= last; ++b) best = max_nan(best, __ldcg(part_at(b) + L::kRows * D + row));
-      float weight_sum = 0.0f, value[kEach];
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) value[i] = 0.0f;
+  if (warp == kWarps) {
+    // Given up: leave only after the copies in flight have landed.
+    if (failed)
+      for (int64_t n = fed > L::kStages ? fed - L::kStages : 0; n < fed; ++n)
+        tc::wait_phase(full + static_cast<int>(n % L::kStages) * 8, static_cast<uint32_t>(n / L::kStages) & 1, nullptr);
+    return;
+  }
+  if (pieces == 0) return;
+
+  // A block has at most two units that it shares, the first and the last of its
+  // stretch.  Their results are announced together at the end: one release,
+  // and no wait in between.  The block that arrives last at a unit joins it.
+  consumers_sync();
+  if (threadIdx.x < pieces) {
+    const Segment &of = control.pending[threadIdx.x];
+    const int64_t first = divide(of.unit_start, share), last = divide(of.unit_start + of.unit_tiles - 1, share);
+    uint32_t before_me;
+    // Releases this block's results (after the barrier) and acquires the others'.
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
+                 : "=r"(before_me)
+                 : "l"(p.counters + first)
+                 : "memory");
+    const bool joins = before_me == static_cast<uint32_t>(last - first);
+    if (joins) p.counters[first] = 0;  // as the next call expects it
+    control.arrived[threadIdx.x] = joins;
+  }
+  consumers_sync();
+  for (int piece = 0; piece < pieces; ++piece) {
+    if (!control.arrived[piece]) continue;
+    s = control.pending[piece];
+    const int64_t first = divide(s.unit_start, share), last = divide(s.unit_start + s.unit_tiles - 1, share);
+    const int32_t parts = static_cast<int32_t>(last - first) + 1;
+    const int32_t rows_here = min(L::kRows, s.tokens * p.groups - s.row0);
+    constexpr int64_t kPart = L::kRows * (D + 2);
+    // Part 0 is the first block's second result, part i > 0 the first result of
+    // block first + i.
+    const float *from = p.partials + (first * 2) * kPart;
+    auto part_at = [&](int32_t i) { return from + (2 * static_cast<int64_t>(i) + (i == 0 ? 1 : 0)) * kPart; };
+    // Maxima and sums: thread (row, every kAcrossth part), joined over shared memory.
+    constexpr int kApart = kWarps * 32 / L::kRows;
+    constexpr int kHeld = (kWarps * 8 * L::kPitch - 2 * kWarps * 32) / L::kRows;  // parts whose maxima are kept
+    float *joined = scratch + kHeld * L::kRows;
+    const int own_row = threadIdx.x % L::kRows;
+    float best = -INFINITY, weight_sum = 0.0f;
 #pragma unroll 4
-      for (int64_t b = first; b <= last; ++b) {
-        const float *from = part_at(b);
-        const float m = __ldcg(from + L::kRows * D + row);
-        const float weight = m == -INFINITY ? 0.0f : exp2_fast(m - best);
-        weight_sum = fmaf(weight, __ldcg(from + L::kRows * (D + 1) + row), weight_sum);
-#pragma unroll
-        for (int i = 0; i < kEach; i += 4) {
-          const float4 x = __ldcg(reinterpret_cast<const float4 *>(from + row * D + channel + i));
-          value[i] = fmaf(weight, x.x, value[i]);
-          value[i + 1] = fmaf(weight, x.y, value[i + 1]);
-          value[i + 2] = fmaf(weight, x.z, value[i + 2]);
-          value[i + 3] = fmaf(weight, x.w, value[i + 3]);
-        }
-      }
-      const int32_t query_row = s.row0 + row;
-      const int64_t index = static_cast<int64_t>(s.first_token + query_row / p.groups) * query_heads +
-                            static_cast<int64_t>(head) * p.groups + query_row % p.groups;
-      const float inverse = weight_sum == 0.0f ? 0.0f : 1.0f / weight_sum;
-      T result[kEach];
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) result[i] = from_float<T>(value[i] * inverse);
-      if constexpr (kEach == 8)
-        *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + index * D + channel) = *reinterpret_cast<uint4 *>(result);
-      else
-        *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + index * D + channel) = *reinterpret_cast<uint2 *>(result);
-      if (channel == 0)
-        p.lse[index] = weight_sum == 0.0f ? -INFINITY : (best + log2f(weight_sum)) * 0.693147180559945f;
+    for (int32_t i = threadIdx.x / L::kRows; i < parts; i += kApart) {
+      const float m = __ldcg(part_at(i) + L::kRows * D + own_row), l = __ldcg(part_at(i) + L::kRows * (D + 1) + own_row);
+      if (i < kHeld) scratch[i * L::kRows + own_row] = m;
+      add_part(best, weight_sum, m, l);
     }
+    joined[threadIdx.x] = best;
+    joined[kWarps * 32 + threadIdx.x] = weight_sum;
+    consumers_sync();
+    best = -INFINITY, weight_sum = 0.0f;
+    for (int i = own_row; i < kWarps * 32; i += L::kRows)
+      add_part(best, weight_sum, joined[i], joined[kWarps * 32 + i]);
+    if (threadIdx.x < L::kRows) {
+      stat_top[own_row] = best;
+      stat_sum[own_row] = weight_sum;
+      if (own_row < rows_here) p.lse[out_row(p, s, s.row0 + own_row)] = natural(best, weight_sum);
+    }
+    consumers_sync();
+    // The outputs, four channels a thread at a time.
+    for (int item = threadIdx.x; item < rows_here * (D / 4); item += kWarps * 32) {
+      const int row = item / (D / 4), channel = item % (D / 4) * 4;
+      const float top = stat_top[row];
+      float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+      for (int32_t i = 0; i < parts; ++i) {
+        const float *part = part_at(i);
+        const float4 x = __ldcg(reinterpret_cast<const float4 *>(part + row * D + channel));
+        const float m = i < kHeld ? scratch[i * L::kRows + row] : __ldcg(part + L::kRows * D + row);
+        const float w = m == -INFINITY ? 0.0f : exp2_fast(m - top);
+        value.x = fmaf(w, x.x, value.x);
+        value.y = fmaf(w, x.y, value.y);
+        value.z = fmaf(w, x.z, value.z);
+        value.w = fmaf(w, x.w, value.w);
+      }
+      const float inverse = stat_sum[row] == 0.0f ? 0.0f : 1.0f / stat_sum[row];
+      __align__(8) const T result[4] = {from_float<T>(value.x * inverse), from_float<T>(value.y * inverse),
+                                        from_float<T>(value.z * inverse), from_float<T>(value.w * inverse)};
+      *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + out_row(p, s, s.row0 + row) * D + channel) =
+          *reinterpret_cast<const uint2 *>(result);
+    }
+    consumers_sync();  // before the next piece writes over the statistics
   }
 }
 
@@ -1008,6 +1173,9 @@ extern "C" int lrk_paged_attention(const lrk_pages *pages, const int32_t *table,
   LRK_REQUIRE(aligned(queries->data, 16) && queries->token_stride % 8 == 0 && queries->head_stride % 8 == 0 &&
                   aligned(out, 16),
               "paged attention: rows must be 16-byte aligned");
+  // Positions among all units' tiles stay far inside 64 bits, shares inside 32.
+  LRK_REQUIRE(static_cast<double>(tokens) * query_heads / 8 * (static_cast<double>(table_width) * pages->page_size / kTile + 1) < 1e12,
+              "paged attention: too many query rows for the table's length");
   LRK_REQUIRE(sequences * heads <= INT32_MAX && tokens * (query_heads / heads) <= INT32_MAX / 2,
               "paged attention: too many slots or query rows");
   if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < lrk_paged_attention_workspace_bytes())
@@ -1027,6 +1195,8 @@ extern "C" int lrk_paged_attention(const lrk_pages *pages, const int32_t *table,
   p.query_head = queries->head_stride;
   p.heads = static_cast<int>(heads);
   p.groups = static_cast<int>(query_heads / heads);
+  p.by_heads = Divider::of(static_cast<uint32_t>(heads));
+  p.by_groups = Divider::of(static_cast<uint32_t>(p.groups));
   p.scale_log2 = scale * 1.44269504088896f;
   p.causal = causal != 0;
   p.out = out;

@@ -221,6 +221,18 @@ def test_attention_long_and_ragged(cuda, bits, dtype, dim, group):
 
 
 @pytest.mark.parametrize("bits,dtype,dim,group", FORMATS)
+@pytest.mark.parametrize("page,groups", [(16, 2), (64, 12), (128, 30)])
+def test_attention_many_tiles_a_block(cuda, bits, dtype, dim, group, page, groups):
+    """Enough rows that every block's ring of tiles goes round many times, over ends of slots."""
+    lengths = [3000 + 997 * (i % 5) + i for i in range(64)]
+    lengths[7], lengths[20], lengths[21] = 0, 1, 40000
+    case = Case(cuda, bits, dtype, dim, group, page, 4, lengths, seed=page)
+    queries = queries_of(case, [1] * 16, groups)
+    out, lse = case.attend(queries, [1] * 16)
+    case.check(queries, [1] * 16, out, lse)
+
+
+@pytest.mark.parametrize("bits,dtype,dim,group", FORMATS)
 def test_attention_window_of_queries(cuda, bits, dtype, dim, group):
     """A chunk of 250 tokens at the end of a longer slot."""
     case = Case(cuda, bits, dtype, dim, group, 64, 1, [1500], seed=4)
