@@ -101,8 +101,8 @@ struct Layout {
   // Blocks on an SM, by registers (NT = 1: 96 a thread for 4-bit rows, 128 for
   // 16-bit ones), and as many stages as their share of shared memory holds.
   static constexpr int kBlocksPerSm = NT == 1 ? (GROUP ? 4 : D == 128 ? 2 : 3) : (NT == 2 ? 2 : 1);
-  static constexpr int kControl = 256;  // bytes of Control
-  static constexpr int kFixed = kScratch + kQuery + kGroups * kRows * 8 + kRows * 4 + 2 * kWarps * kRows * 4 + 2 * 16 * 8 +
+  static constexpr int kControl = 416;  // bytes of Control
+  static constexpr int kFixed = kScratch + kQuery + kGroups * kRows * 8 + kRows * 8 + 2 * kWarps * kRows * 4 + 2 * 16 * 8 +
                                 kControl;
   static constexpr int kFit = ((232448 / kBlocksPerSm - 1024) / 128 * 128 - kFixed) / kStage;
   // A multiple of the warps, so that a stage always falls to the same warp: it
@@ -113,7 +113,8 @@ struct Layout {
   static constexpr int kQueryAt = kScratchAt + kScratch;
   static constexpr int kSumsAt = kQueryAt + kQuery;
   static constexpr int kFactorAt = kSumsAt + kGroups * kRows * 8;
-  static constexpr int kStatsAt = kFactorAt + kRows * 4;
+  static constexpr int kSeenAt = kFactorAt + kRows * 4;
+  static constexpr int kStatsAt = kSeenAt + kRows * 4;
   static constexpr int kBarriersAt = kStatsAt + 2 * kWarps * kRows * 4;
   static constexpr int kBytes = kBarriersAt + 2 * kStages * 8 + kControl;
   static_assert(kStages >= kWarps, "every warp needs a stage of its own");
@@ -193,6 +194,16 @@ __device__ __forceinline__ bool wait(uint32_t barrier, uint32_t parity, volatile
   return done || tc::wait_phase(barrier, parity, abort);
 }
 
+// A barrier of the consumers that tells all of them whether `x` holds for any.
+__device__ __forceinline__ bool consumers_any(bool x) {
+  uint32_t any;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, %2, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(any)
+      : "r"(static_cast<uint32_t>(x)), "n"(kWarps * 32)
+      : "memory");
+  return any;
+}
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
 
 // a / b for a >= 0, b > 0.  Out of line: the 64-bit division is some hundred
@@ -278,6 +289,8 @@ struct Control {
   int32_t abort;
   int32_t arrived[2];
   Segment pending[2];
+  uint64_t posted[2], taken[2];  // barriers of the two segments below
+  Segment segments[2];           // from the feeding warp to the consumers; slot -1 ends them
 };
 
 template <typename T, int D, int GROUP, int NT>
@@ -302,7 +315,6 @@ struct Consumer {
   float offset_sum[NT][kNG][2];
   float scaled_sum[NT][(kNG + 1) / 2][4];  // of group gi: elements 2 (gi mod 2) and after
   float factor[NT][2];
-  int32_t seen[NT][2];
 
   __device__ __forceinline__ void clear() {
     lift = 0.0f;
@@ -449,7 +461,8 @@ struct Consumer {
   // Adds 16 rows' weighted values to the output.  With MASKED, rows that a
   // query does not see add nothing, whatever their scales hold.
   template <bool MASKED>
-  __device__ __forceinline__ void values(const uint8_t *stage, int half, int lane, const float (*w)[4], int32_t first_row) {
+  __device__ __forceinline__ void values(const uint8_t *stage, int half, int lane, const float (*w)[4], int32_t first_row,
+                                         const int32_t *seen_by) {
     const int g = lane >> 2, t = lane & 3;
     const uint8_t *values_at = stage + L::kCodes + L::kScales;
     if constexpr (GROUP == 0) {
@@ -491,7 +504,7 @@ struct Consumer {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float2 v = i < 2 ? v0 : v1;
-            const bool none = MASKED && first_row + row + (i < 2 ? 0 : 8) >= seen[nt][i & 1];
+            const bool none = MASKED && first_row + row + (i < 2 ? 0 : 8) >= seen_by[nt * 8 + 2 * t + (i & 1)];
             scaled[i] = none ? 0.0f : w[nt][i] * v.x;
             float &sum_of = offset_sum[nt][gi][i & 1];
             sum_of = none ? sum_of : fmaf(w[nt][i], v.y, sum_of);
@@ -530,7 +543,7 @@ struct Consumer {
 
   template <bool MASKED>
   __device__ __forceinline__ void tile(uint8_t *stage, const uint8_t *query_at, const float *group_sums, int lane,
-                                       int32_t first_row, int32_t seen_max) {
+                                       int32_t first_row, int32_t seen_max, const int32_t *seen_by) {
     float s[2][NT][4];
     const float lifted = lift;
     if constexpr (GROUP != 0) check_scales(stage, lane);
@@ -544,7 +557,7 @@ struct Consumer {
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (row + half * 16 + (i < 2 ? 0 : 8) >= seen[nt][i & 1]) s[half][nt][i] = -INFINITY;
+            if (row + half * 16 + (i < 2 ? 0 : 8) >= seen_by[nt * 8 + 2 * (lane & 3) + (i & 1)]) s[half][nt][i] = -INFINITY;
     }
     bool grows = lift != lifted;
     float best[NT][2];
@@ -602,7 +615,7 @@ struct Consumer {
       __syncwarp();
     }
 #pragma unroll
-    for (int half = 0; half < 2; ++half) values<MASKED>(stage, half, lane, s[half], first_row);
+    for (int half = 0; half < 2; ++half) values<MASKED>(stage, half, lane, s[half], first_row, seen_by);
   }
 };
 
@@ -667,6 +680,10 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
       tc::init_barrier(full + i * 8, 1);
       tc::init_barrier(empty + i * 8, 1);
     }
+    for (int i = 0; i < 2; ++i) {
+      tc::init_barrier(shared_address(&control.posted[i]), 1);
+      tc::init_barrier(shared_address(&control.taken[i]), 1);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     *abort = 0;
   }
@@ -720,27 +737,24 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
   walk.slot_start = control.slot_start;
   walk.slot = control.slot;
 
-  // The feeding warp's place in the ring, or a consumer's next tile of it.
-  int stage = warp == kWarps ? 0 : warp;
-  uint32_t phase = 0;
-  int64_t fed = 0;
-  bool failed = false;
-  Consumer<T, D, GROUP, NT> c;
-  float *group_sums = reinterpret_cast<float *>(shared + L::kSumsAt);
-  float *factors = reinterpret_cast<float *>(shared + L::kFactorAt);
-  float *stat_top = reinterpret_cast<float *>(shared + L::kStatsAt), *stat_sum = stat_top + kWarps * L::kRows;
-  float *scratch = reinterpret_cast<float *>(shared + L::kScratchAt);
-  const uint8_t *query_at = shared + L::kQueryAt;
-  const int g = lane >> 2, t = lane & 3;
-  // A negative scale is taken by the queries, so that the largest score is the
-  // largest product; the factor stays above zero for the sake of -inf.
-  const uint32_t turn = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
-  constexpr float kLeastFactor = 1e-37f;
-  int pieces = 0;
-  int turn_of = 0;  // the warp that the segment's first tile falls to
-
-  while (walk.next(p, s)) {
-    if (warp == kWarps) {
+  if (warp == kWarps) {
+    int stage = 0;
+    uint32_t phase = 0;
+    int64_t fed = 0;
+    bool failed = false;
+    for (int number = 0;; ++number) {
+      const bool more = walk.next(p, s);
+      if (!more) s.slot = -1;
+      const int at_segment = number & 1;
+      const bool taken = number < 2 || wait(shared_address(&control.taken[at_segment]), ((number >> 1) & 1) ^ 1, abort);
+      failed = __any_sync(0xffffffffu, !taken);
+      if (failed) break;
+      if (lane == 0) {
+        control.segments[at_segment] = s;
+        tc::arrive(shared_address(&control.posted[at_segment]));  // releases the segment
+      }
+      __syncwarp();
+      if (!more) break;
       // The feeding warp: every tile of the stretch in order, through the ring.
       const int32_t *entries = p.table + static_cast<int64_t>(s.slot) * p.table_stride;
       for (int32_t first = s.tile0; first < s.tile1 && !failed; first += 32) {
@@ -749,7 +763,8 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
         const int parts = p.pages.page_size == 16 ? 2 : 1;
         const int rows = parts == 1 ? kTile : 16;  // of a part
         int copies = 0;                            // parts that the tile's visible rows lie in
-        int64_t y[2] = {0, 0};
+        const uint8_t *from[2][4];                 // 4-bit: key rows, key scales, value rows, value scales
+        int32_t y[2] = {0, 0};                     // 16-bit: the row among all pages'
         if (first + lane < s.tile1) {
           copies = parts == 1 || row + 16 >= s.seen_max ? 1 : 2;
 #pragma unroll
@@ -760,7 +775,12 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
                 page = 0;
                 atomicOr(p.flag, kFlagRow);
               }
-              y[part] = static_cast<int64_t>(page) * p.pages.page_size + (row & (p.pages.page_size - 1));
+              const int64_t at = static_cast<int64_t>(page) * p.pages.page_size + (row & (p.pages.page_size - 1));
+              y[part] = static_cast<int32_t>(at);
+              from[part][0] = p.pages.keys + at * L::kRowBytes;
+              from[part][1] = reinterpret_cast<const uint8_t *>(p.pages.key_scales) + at * L::kScaleBytes;
+              from[part][2] = p.pages.values + at * L::kRowBytes;
+              from[part][3] = reinterpret_cast<const uint8_t *>(p.pages.value_scales) + at * L::kScaleBytes;
             }
         }
         const int32_t here = min(32, s.tile1 - first);
@@ -771,30 +791,27 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
             given_up = fed >= L::kStages && !wait(empty + stage * 8, phase ^ 1, abort);
             if (!given_up) {
               tc::expect_bytes(barrier, copies * rows * (L::kStage / kTile));
-              for (int part = 0; part < copies; ++part) {
-                const int64_t from = y[part];
 #pragma unroll
-                for (int side = 0; side < 2; ++side) {
-                  const uint32_t to = at + side * (L::kCodes + L::kScales);
-                  if constexpr (GROUP == 0) {
+              for (int part = 0; part < 2; ++part)
+                if (part < copies)
 #pragma unroll
-                    for (int box = 0; box < D / 64; ++box)  // 64 channels wide
-                      tc::tma_box(to + box * (kTile * 128) + part * 16 * 128, side ? &value_map : &key_map, box * 64,
-                                  static_cast<int>(from), barrier);
-                  } else {
-                    bulk_copy(to + part * 16 * L::kRowBytes, (side ? p.pages.values : p.pages.keys) + from * L::kRowBytes,
-                              rows * L::kRowBytes, barrier);
-                    bulk_copy(to + L::kCodes + part * 16 * L::kScaleBytes,
-                              (side ? p.pages.value_scales : p.pages.key_scales) + from * L::kGroups,
-                              rows * L::kScaleBytes, barrier);
+                  for (int side = 0; side < 2; ++side) {
+                    const uint32_t to = at + side * (L::kCodes + L::kScales);
+                    if constexpr (GROUP == 0) {
+#pragma unroll
+                      for (int box = 0; box < D / 64; ++box)  // 64 channels wide
+                        tc::tma_box(to + box * (kTile * 128) + part * 16 * 128, side ? &value_map : &key_map, box * 64,
+                                    y[part], barrier);
+                    } else {
+                      bulk_copy(to + part * 16 * L::kRowBytes, from[part][2 * side], rows * L::kRowBytes, barrier);
+                      bulk_copy(to + L::kCodes + part * 16 * L::kScaleBytes, from[part][2 * side + 1],
+                                rows * L::kScaleBytes, barrier);
+                    }
                   }
-                }
-              }
             }
           }
           // The warp stays together: a lane that ran ahead would find an older
           // phase of its stage's barrier with the parity that it waits for.
-          if (given_up) atomicOr(p.flag, kFlagTimeout);
           failed = __any_sync(0xffffffffu, given_up || *abort);
           if (failed) break;
           ++fed;
@@ -805,9 +822,43 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
         }
       }
       if (failed) break;
-      continue;
     }
+    // Given up: leave only after the copies in flight have landed.
+    if (failed) {
+      if (lane == 0) atomicOr(p.flag, kFlagTimeout);
+      for (int64_t n = fed > L::kStages ? fed - L::kStages : 0; n < fed; ++n)
+        tc::wait_phase(full + static_cast<int>(n % L::kStages) * 8, static_cast<uint32_t>(n / L::kStages) & 1, nullptr);
+    }
+    return;
+  }
 
+  Consumer<T, D, GROUP, NT> c;
+  float *group_sums = reinterpret_cast<float *>(shared + L::kSumsAt);
+  float *factors = reinterpret_cast<float *>(shared + L::kFactorAt);
+  int32_t *seen_by = reinterpret_cast<int32_t *>(shared + L::kSeenAt);
+  float *stat_top = reinterpret_cast<float *>(shared + L::kStatsAt), *stat_sum = stat_top + kWarps * L::kRows;
+  float *scratch = reinterpret_cast<float *>(shared + L::kScratchAt);
+  const uint8_t *query_at = shared + L::kQueryAt;
+  const int g = lane >> 2, t = lane & 3;
+  // A negative scale is taken by the queries, so that the largest score is the
+  // largest product; the factor stays above zero for the sake of -inf.
+  const uint32_t turn = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
+  constexpr float kLeastFactor = 1e-37f;
+  int pieces = 0;
+  int stage = warp;  // of this warp's next tile
+  uint32_t phase = 0;
+  int turn_of = 0;   // the warp that the segment's first tile falls to
+
+  for (int number = 0;; ++number) {
+    const int at_segment = number & 1;
+    const bool posted = wait(shared_address(&control.posted[at_segment]), (number >> 1) & 1, abort);
+    if (consumers_any(!posted)) {  // all warps go on or none
+      *abort = 1;
+      if (threadIdx.x == 0) atomicOr(p.flag, kFlagTimeout);
+      return;
+    }
+    const Segment &s = control.segments[at_segment];
+    if (s.slot < 0) break;
     const int32_t head = s.slot - s.sequence * p.heads;
     const int32_t rows_total = s.tokens * p.groups;
     // Query fragments: the B operand of a k-step holds, for query row g, the
@@ -817,6 +868,7 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
     for (int row = threadIdx.x / kAcross; row < L::kRows; row += kWarps * 32 / kAcross) {
       const int32_t query_row = s.row0 + row;
       const bool live = query_row < rows_total;
+      if (column == 0) seen_by[row] = live ? rows_seen(p, s, query_row) : s.seen_max;
       const T *from = static_cast<const T *>(p.queries) +
                       static_cast<int64_t>(s.first_token + (live ? p.by_groups(query_row) : 0)) * p.query_token +
                       (static_cast<int64_t>(head) * p.groups + (live ? query_row - p.by_groups(query_row) * p.groups : 0)) * p.query_head;
@@ -877,24 +929,22 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int32_t row = s.row0 + nt * 8 + 2 * t + i;
         c.factor[nt][i] = factors[nt * 8 + 2 * t + i];
-        c.seen[nt][i] = row < rows_total ? rows_seen(p, s, row) : s.seen_max;
       }
     c.clear();
-    const int32_t tiles = max(s.tile1 - s.tile0, 0);
+    const int32_t tile0 = s.tile0, tiles = max(s.tile1 - s.tile0, 0), seen_min = s.seen_min;
     // The stretch's tiles go to the warps in turn.
     for (int32_t i = (warp - turn_of) & (kWarps - 1); i < tiles; i += kWarps) {
       uint8_t *const at = shared + stage * L::kStage;
       const bool landed = wait(full + stage * 8, phase, abort);
-      const int32_t first_row = (s.tile0 + i) * kTile;
+      const int32_t first_row = (tile0 + i) * kTile;
       if (!landed) {  // every barrier below is still met
         if (lane == 0) atomicOr(p.flag, kFlagTimeout);
-      } else if (first_row + kTile > s.seen_min) {
-        c.template tile<true>(at, query_at, group_sums, lane, first_row, s.seen_max);
+      } else if (first_row + kTile > seen_min) {
+        c.template tile<true>(at, query_at, group_sums, lane, first_row, s.seen_max, seen_by);
         if constexpr (GROUP == 0) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       } else {
-        c.template tile<false>(at, query_at, group_sums, lane, first_row, s.seen_max);
+        c.template tile<false>(at, query_at, group_sums, lane, first_row, s.seen_max, seen_by);
       }
       __syncwarp();
       if (lane == 0) tc::arrive(empty + stage * 8);
@@ -1010,14 +1060,8 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
       if (threadIdx.x == 0) control.pending[pieces] = s;
       ++pieces;
     }
-  }
-
-  if (warp == kWarps) {
-    // Given up: leave only after the copies in flight have landed.
-    if (failed)
-      for (int64_t n = fed > L::kStages ? fed - L::kStages : 0; n < fed; ++n)
-        tc::wait_phase(full + static_cast<int>(n % L::kStages) * 8, static_cast<uint32_t>(n / L::kStages) & 1, nullptr);
-    return;
+    consumers_sync();
+    if (threadIdx.x == 0) tc::arrive(shared_address(&control.taken[at_segment]));
   }
   if (pieces == 0) return;
 
@@ -1041,7 +1085,7 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
   consumers_sync();
   for (int piece = 0; piece < pieces; ++piece) {
     if (!control.arrived[piece]) continue;
-    s = control.pending[piece];
+    const Segment &s = control.pending[piece];
     const int64_t first = divide(s.unit_start, share), last = divide(s.unit_start + s.unit_tiles - 1, share);
     const int32_t parts = static_cast<int32_t>(last - first) + 1;
     const int32_t rows_here = min(L::kRows, s.tokens * p.groups - s.row0);
