@@ -300,24 +300,28 @@ struct Consumer {
   static constexpr int kNG = L::kGroups;
   using P = std::conditional_t<GROUP == 0, T, __half>;  // the weights' type, as the matrix instruction wants V's
 
-  // Weights are exp2(s - top): top is the running maximum less kHead, so that
-  // small weights stay in f16's normal range (a weight is rounded to 11 bits
-  // down to 2^-26 of the largest; with kHead = 0 it would be 2^-14, which cost
-  // a third of a bf16 output's precision over 34,768 rows).  For 4-bit rows the
-  // operand is weight * scale: 2^12 * 8 = 2^15 while a value's scale is at most
-  // 8; `lift` (0 until then) raises top where a larger one is met.
-  static constexpr float kHead = GROUP == 0 ? (sizeof(P) == 2 && std::is_same<P, __half>::value ? 14.0f : 0.0f) : 12.0f;
-  static constexpr uint32_t kPlainScale = 0x4800;  // 8.0 in f16
+  // Weights are exp2(s - top).  top follows the running maximum loosely: it is
+  // set to the maximum less kHead, and set again only when a score passes it by
+  // more than kMost.  So most tiles neither exchange maxima nor rescale (with
+  // an exact maximum 11 of a warp's first 18 tiles did), and small weights stay
+  // in f16's normal range (11 bits down to 2^-22 of the largest; with kHead = 0
+  // it would be 2^-14, which cost a third of a bf16 output's precision over
+  // 34,768 rows).  For 4-bit rows the operand is weight * scale: 2^12 * 8 = 2^15
+  // while a value's scale is at most 8; `lift` (0 until then) raises top where
+  // a larger one is met.  bf16 has float32's range and needs no head.
+  static constexpr bool kHalfWeights = std::is_same<P, __half>::value;
+  static constexpr float kHead = GROUP ? 8.0f : kHalfWeights ? 10.0f : 0.0f;
+  static constexpr float kMost = GROUP ? 12.0f : kHalfWeights ? 14.0f : 8.0f;
 
   float out[kOut][NT][4];
   float top[NT][2], sum[NT][2];
-  float lift;
+  int32_t lift;
   float offset_sum[NT][kNG][2];
   float scaled_sum[NT][(kNG + 1) / 2][4];  // of group gi: elements 2 (gi mod 2) and after
   float factor[NT][2];
 
   __device__ __forceinline__ void clear() {
-    lift = 0.0f;
+    lift = 0;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -343,20 +347,54 @@ struct Consumer {
     load_words<4>(query_at + ((nt * (D / 32) + pair) * 32 + lane) * 16, b);
   }
 
-  // Raises `lift` where a value's scale in this tile asks for it.  Rows that
-  // are not visible may hold anything; they can only raise it too far.
-  __device__ __forceinline__ void check_scales(const uint8_t *stage, int lane) {
+  // The largest of the value scales' bits in this lane's row of the tile.  Rows
+  // that are not visible may hold anything; they can only raise `lift` too far.
+  __device__ __forceinline__ static uint32_t largest_scale(const uint8_t *stage, int lane) {
     uint32_t w[kNG], largest = 0;
     load_words<kNG>(stage + 2 * L::kCodes + L::kScales + lane * L::kScaleBytes, w);
 #pragma unroll
     for (int gi = 0; gi < kNG; ++gi) largest = max(largest, w[gi] & 0xffffu);
-    if (!__any_sync(0xffffffffu, largest > kPlainScale)) return;
-    uint32_t exponent = 0;  // f16's, of the largest finite scale
+    return largest;
+  }
+
+  // The largest scale (in f16's bits) that the lift allows: 8 * 2^lift.
+  __device__ __forceinline__ uint32_t plain_scale() const { return 0x4800u + (static_cast<uint32_t>(lift) << 10); }
+
+  // Sets top anew for scores whose maxima in this lane are `best`.
+  __device__ __forceinline__ void raise(const float (*best)[2], uint32_t largest) {
+    const int32_t lifted = lift;
+    if constexpr (GROUP != 0) {
+      if (__any_sync(0xffffffffu, largest > plain_scale())) {
+        // NaN scales (0x7fff) reach their own weights alone, whatever the lift.
+        const uint32_t exponent = __reduce_max_sync(0xffffffffu, largest < 0x7c00u ? largest >> 10 : 0x1eu);
+        lift = max(lift, static_cast<int32_t>(exponent) - 17);  // scale < 2^(exponent - 14)
+      }
+    }
 #pragma unroll
-    for (int gi = 0; gi < kNG; ++gi)
-      if ((w[gi] & 0xffffu) < 0x7c00u) exponent = max(exponent, (w[gi] & 0xffffu) >> 10);
-    exponent = __reduce_max_sync(0xffffffffu, exponent);
-    lift = fmaxf(lift, static_cast<float>(static_cast<int>(exponent) - 17));  // scale < 2^(exponent - 14)
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        // max_nan: a NaN score makes the result NaN.
+        float m = best[nt][i];
+        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 4));
+        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 8));
+        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        const float next = max_nan(fmaf(m, factor[nt][i], static_cast<float>(lift) - kHead),
+                                   top[nt][i] + static_cast<float>(lift - lifted));
+        const float keep = top[nt][i] == -INFINITY ? 0.0f : exp2_fast(top[nt][i] - next);
+        top[nt][i] = next;
+        sum[nt][i] *= keep;
+#pragma unroll
+        for (int g = 0; g < kNG; ++g) {
+          offset_sum[nt][g][i] *= keep;
+          scaled_sum[nt][g / 2][i + 2 * (g & 1)] *= keep;
+        }
+#pragma unroll
+        for (int m = 0; m < kOut; ++m) {
+          out[m][nt][i] *= keep;
+          out[m][nt][i + 2] *= keep;
+        }
+      }
   }
 
   // Scores of the tile's rows against the block's query rows, both halves of 16
@@ -545,8 +583,6 @@ struct Consumer {
   __device__ __forceinline__ void tile(uint8_t *stage, const uint8_t *query_at, const float *group_sums, int lane,
                                        int32_t first_row, int32_t seen_max, const int32_t *seen_by) {
     float s[2][NT][4];
-    const float lifted = lift;
-    if constexpr (GROUP != 0) check_scales(stage, lane);
     scores(stage, query_at, group_sums, lane, s);
     if constexpr (MASKED) {
       const int g = lane >> 2;
@@ -559,40 +595,18 @@ struct Consumer {
           for (int i = 0; i < 4; ++i)
             if (row + half * 16 + (i < 2 ? 0 : 8) >= seen_by[nt * 8 + 2 * (lane & 3) + (i & 1)]) s[half][nt][i] = -INFINITY;
     }
-    bool grows = lift != lifted;
+    uint32_t largest = 0;
+    if constexpr (GROUP != 0) largest = largest_scale(stage, lane);
+    bool raises = largest > plain_scale();
     float best[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        // max_nan: a NaN score makes the maximum, and with it the result, NaN.
-        float m = max_nan(max_nan(s[0][nt][i], s[0][nt][i + 2], s[1][nt][i]), s[1][nt][i + 2]);
-        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 4));
-        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 8));
-        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 16));
-        best[nt][i] = max_nan(fmaf(m, factor[nt][i], lift - kHead), top[nt][i] + (lift - lifted));
-        grows |= best[nt][i] != top[nt][i];
+        best[nt][i] = max_nan(max_nan(s[0][nt][i], s[0][nt][i + 2], s[1][nt][i]), s[1][nt][i + 2]);
+        raises |= fmaf(best[nt][i], factor[nt][i], static_cast<float>(lift) - kMost) > top[nt][i];
       }
-    if (__any_sync(0xffffffffu, grows)) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float keep = top[nt][i] == -INFINITY ? 0.0f : exp2_fast(top[nt][i] - best[nt][i]);
-          top[nt][i] = best[nt][i];
-          sum[nt][i] *= keep;
-#pragma unroll
-          for (int g = 0; g < kNG; ++g) {
-            offset_sum[nt][g][i] *= keep;
-            scaled_sum[nt][g / 2][i + 2 * (g & 1)] *= keep;
-          }
-#pragma unroll
-          for (int m = 0; m < kOut; ++m) {
-            out[m][nt][i] *= keep;
-            out[m][nt][i + 2] *= keep;
-          }
-        }
-    }
+    if (__any_sync(0xffffffffu, raises)) raise(best, largest);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

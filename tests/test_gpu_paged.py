@@ -55,7 +55,8 @@ def rotate(x, table, positions, interleaved):
 class Case:
     """Pages with every unused byte poisoned, a shuffled page table (a strided view), and the rows' float64 values."""
 
-    def __init__(self, device, bits, dtype, dim, group, page, heads, lengths, seed=0, spare=3, key_spread=1.0):
+    def __init__(self, device, bits, dtype, dim, group, page, heads, lengths, seed=0, spare=3, key_spread=1.0,
+                 value_spread=None):
         import torch
 
         from code_for_iclr27_b200.paged import Pages
@@ -91,6 +92,8 @@ class Case:
             held = []
             for side, pool in enumerate((keys, values)):
                 x = self.rng.standard_normal((n, dim)).astype(np.float32) * (key_spread if side == 0 else 1.0)
+                if side == 1 and value_spread is not None:
+                    x = np.clip(x * value_spread(n)[:, None].astype(np.float32), -65000, 65000)  # finite in float16
                 pages, lines = table[s, np.arange(n) // page], np.arange(n) % page
                 if bits == 16:
                     x = torch.from_numpy(x).to(self.dtype)
@@ -250,6 +253,19 @@ def test_attention_peaked_and_large_scores(cuda, bits, dtype, dim, group):
     for scale in (None, -0.5, 0.0):
         out, lse = case.attend(queries, [1], scale=scale)
         case.check(queries, [1], out, lse, scale=scale)
+
+
+@pytest.mark.parametrize("bits,dtype,dim,group", FORMATS)
+@pytest.mark.parametrize("large", [60.0, 4000.0, 15000.0])
+def test_attention_value_magnitudes(cuda, bits, dtype, dim, group, large):
+    """Values whose 4-bit scales grow along the rows, up to near float16's largest; few large ones among small ones."""
+    rising = lambda n: large * (np.arange(n) + 1.0) / max(n, 1)  # noqa: E731
+    some = lambda n: np.where(np.arange(n) % 97 == 50, large, 1e-3)  # noqa: E731
+    for spread in (rising, some):
+        case = Case(cuda, bits, dtype, dim, group, 32, 1, [700, 40], seed=13, value_spread=spread)
+        queries = queries_of(case, [1, 1], 4)
+        out, lse = case.attend(queries, [1, 1])
+        case.check(queries, [1, 1], out, lse)
 
 
 @pytest.mark.parametrize("bits,dtype,dim,group", [(16, "f16", 128, 0), (16, "bf16", 64, 0), (4, "bf16", 128, 64), (4, "f16", 64, 32)])
