@@ -46,8 +46,8 @@ namespace {
 using namespace paged;
 
 constexpr int kTile = 32;   // rows per tile
-constexpr int kWarps = 4;   // consumer warps; one more feeds them
-constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
 constexpr int kMinTiles = kWarps;  // tiles per block, at least
 constexpr int kCounters = 4096;    // workspace: arrival counters, then partial results
 
@@ -98,26 +98,24 @@ struct Layout {
   static constexpr int kPitch = D + 4;
   static constexpr int kScratch = kWarps * 8 * kPitch * 4;
   static constexpr int kQuery = NT * (D / 16) * 32 * 8;
-  // Blocks on an SM, by registers (NT = 1: 96 a thread for 4-bit rows, 128 for
-  // 16-bit ones), and as many stages as their share of shared memory holds.
-  static constexpr int kBlocksPerSm = NT == 1 ? (GROUP ? 4 : D == 128 ? 2 : 3) : (NT == 2 ? 2 : 1);
+  // Blocks on an SM, by registers (4-bit rows: 96, 168 and 255 a thread), and
+  // one or two stages a warp, as their share of shared memory holds.
+  static constexpr int kBlocksPerSm = GROUP ? (NT == 1 ? 5 : NT == 2 ? 3 : 2) : (NT <= 2 ? 3 : 2);
   static constexpr int kControl = 416;  // bytes of Control
-  static constexpr int kFixed = kScratch + kQuery + kGroups * kRows * 8 + kRows * 8 + 2 * kWarps * kRows * 4 + 2 * 16 * 8 +
-                                kControl;
-  static constexpr int kFit = ((232448 / kBlocksPerSm - 1024) / 128 * 128 - kFixed) / kStage;
-  // A multiple of the warps, so that a stage always falls to the same warp: it
-  // has then seen the stage's last phase end, and a parity names one phase.
-  static constexpr int kStages = (kFit > 12 ? 12 : kFit) / kWarps * kWarps;
-  // After the stages: scratch, query fragments, group sums, factors, maxima and sums, barriers.
-  static constexpr int kScratchAt = kStages * kStage;
-  static constexpr int kQueryAt = kScratchAt + kScratch;
+  static constexpr int kFixed = kQuery + kGroups * kRows * 8 + kRows * 8 + 2 * kWarps * kRows * 4 + kControl;
+  static constexpr int kFit = ((232448 / kBlocksPerSm - 1024) / 128 * 128 - kFixed) / kStage / kWarps;
+  static constexpr int kDepth = kFit > 2 ? 2 : kFit;  // stages of a warp
+  static constexpr int kStages = kDepth * kWarps;
+  // The stages, in their place the scratch of a segment's end; query
+  // fragments, group sums, factors, maxima and sums, control.
+  static constexpr int kQueryAt = kStages * kStage > kScratch ? kStages * kStage : kScratch;
   static constexpr int kSumsAt = kQueryAt + kQuery;
   static constexpr int kFactorAt = kSumsAt + kGroups * kRows * 8;
   static constexpr int kSeenAt = kFactorAt + kRows * 4;
   static constexpr int kStatsAt = kSeenAt + kRows * 4;
-  static constexpr int kBarriersAt = kStatsAt + 2 * kWarps * kRows * 4;
-  static constexpr int kBytes = kBarriersAt + 2 * kStages * 8 + kControl;
-  static_assert(kStages >= kWarps, "every warp needs a stage of its own");
+  static constexpr int kControlAt = kStatsAt + 2 * kWarps * kRows * 4;
+  static constexpr int kBytes = kControlAt + kControl;
+  static_assert(kDepth >= 1, "every warp needs a stage of its own");
 };
 
 __device__ __forceinline__ void mma(const __half *, float *d, const uint32_t *a, uint32_t b0, uint32_t b1,
@@ -194,18 +192,6 @@ __device__ __forceinline__ bool wait(uint32_t barrier, uint32_t parity, volatile
   return done || tc::wait_phase(barrier, parity, abort);
 }
 
-// A barrier of the consumers that tells all of them whether `x` holds for any.
-__device__ __forceinline__ bool consumers_any(bool x) {
-  uint32_t any;
-  asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, %2, p;\n selp.u32 %0, 1, 0, q;\n}\n"
-      : "=r"(any)
-      : "r"(static_cast<uint32_t>(x)), "n"(kWarps * 32)
-      : "memory");
-  return any;
-}
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
-
 // a / b for a >= 0, b > 0.  Out of line: the 64-bit division is some hundred
 // instructions that hardly any call needs.
 __device__ __noinline__ int64_t divide_long(int64_t a, int64_t b) { return a / b; }
@@ -281,16 +267,16 @@ struct Walk {
   }
 };
 
-// A block's shared words beside the ring.
+// A block's shared words beside the stages.
+template <int ROWS>
 struct Control {
-  int64_t sums[2][kWarps + 1];
-  int64_t slot_start;
-  int32_t slot;
+  uint64_t landed[2 * kWarps];  // barriers of the stages
+  int64_t sums[2][kWarps];
+  Walk<ROWS> walk;
   int32_t abort;
   int32_t arrived[2];
   Segment pending[2];
-  uint64_t posted[2], taken[2];  // barriers of the two segments below
-  Segment segments[2];           // from the feeding warp to the consumers; slot -1 ends them
+  Segment segments[2];  // this one and the next; slot -1 ends them
 };
 
 template <typename T, int D, int GROUP, int NT>
@@ -656,12 +642,11 @@ __global__ __launch_bounds__(kThreads, (Layout<T, D, GROUP, NT>::kBlocksPerSm))
 void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_constant__ CUtensorMap key_map,
                       const __grid_constant__ CUtensorMap value_map) {
   using L = Layout<T, D, GROUP, NT>;
-  static_assert(sizeof(Control) <= L::kControl, "Control has grown");
+  static_assert(sizeof(Control<L::kRows>) <= L::kControl, "Control has grown");
   extern __shared__ __align__(1024) uint8_t shared[];
   const uint32_t base = shared_address(shared);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t full = base + L::kBarriersAt, empty = full + L::kStages * 8;
-  Control &control = *reinterpret_cast<Control *>(shared + L::kBarriersAt + 2 * L::kStages * 8);
+  Control<L::kRows> &control = *reinterpret_cast<Control<L::kRows> *>(shared + L::kControlAt);
   volatile int *abort = &control.abort;
   if (base & 1023) {  // the 128-byte swizzle goes by address bits
     if (threadIdx.x == 0) atomicOr(p.flag, kFlagTimeout);
@@ -671,179 +656,78 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
   // All slots' tiles and units, and from them the blocks' share.
   const int32_t each = (p.slots + kThreads - 1) / kThreads;
   const int32_t mine0 = min(static_cast<int32_t>(threadIdx.x) * each, p.slots), mine1 = min(mine0 + each, p.slots);
-  int64_t tiles_sum = 0, units_sum = 0;
-  Segment s;
-  int32_t units = 0;
-  for (int32_t i = mine0; i < mine1; ++i) {
-    slot_work<L::kRows>(p, i, s, units);
-    units_sum += units;
-    tiles_sum += static_cast<int64_t>(units) * s.unit_tiles;
-    if (blockIdx.x == 0 && p.lengths[i] > p.capacity) atomicOr(p.flag, kFlagRow);
-  }
-#pragma unroll
-  for (int step = 16; step > 0; step >>= 1) {
-    tiles_sum += __shfl_xor_sync(0xffffffffu, tiles_sum, step);
-    units_sum += __shfl_xor_sync(0xffffffffu, units_sum, step);
-  }
-  if (lane == 0) {
-    control.sums[0][warp] = tiles_sum;
-    control.sums[1][warp] = units_sum;
-  }
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < L::kStages; ++i) {
-      tc::init_barrier(full + i * 8, 1);
-      tc::init_barrier(empty + i * 8, 1);
+  int64_t share;
+  {
+    Segment s;
+    int64_t tiles_sum = 0, units_sum = 0;
+    int32_t units = 0;
+    for (int32_t i = mine0; i < mine1; ++i) {
+      slot_work<L::kRows>(p, i, s, units);
+      units_sum += units;
+      tiles_sum += static_cast<int64_t>(units) * s.unit_tiles;
+      if (blockIdx.x == 0 && p.lengths[i] > p.capacity) atomicOr(p.flag, kFlagRow);
     }
-    for (int i = 0; i < 2; ++i) {
-      tc::init_barrier(shared_address(&control.posted[i]), 1);
-      tc::init_barrier(shared_address(&control.taken[i]), 1);
+#pragma unroll
+    for (int step = 16; step > 0; step >>= 1) {
+      tiles_sum += __shfl_xor_sync(0xffffffffu, tiles_sum, step);
+      units_sum += __shfl_xor_sync(0xffffffffu, units_sum, step);
     }
-    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-    *abort = 0;
-  }
-  __syncthreads();
-  tiles_sum = units_sum = 0;
-#pragma unroll
-  for (int w = 0; w <= kWarps; ++w) {
-    tiles_sum += control.sums[0][w];
-    units_sum += control.sums[1][w];
-  }
-  // With few units a block takes a piece of one unit (a unit rounded up to
-  // whole pieces): sum ceil(tiles / share) <= tiles_sum / share + units <=
-  // grid.  A second unit costs a block its start and its end once more, some
-  // 4 us; rounding costs the blocks units / grid of their time.  So with many
-  // units the shares are equal and cross the units' ends.
-  const bool pieces_apart = units_sum * 4 <= gridDim.x;
-  const int64_t blocks = pieces_apart ? gridDim.x - units_sum : gridDim.x;
-  const int64_t share = lmax(divide(tiles_sum + blocks - 1, blocks), kMinTiles);
-  Walk<L::kRows> walk;
-  walk.round = pieces_apart ? static_cast<int32_t>(share) : 1;
-  int64_t mine = 0;
-  for (int32_t i = mine0; i < mine1; ++i) {
-    if (mine1 - mine0 > 1) slot_work<L::kRows>(p, i, s, units);
-    mine += units * (pieces_apart ? static_cast<int64_t>((s.unit_tiles + walk.round - 1) / walk.round) * walk.round
-                                  : s.unit_tiles);
-  }
-  int64_t before = mine;
-#pragma unroll
-  for (int step = 1; step < 32; step <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, before, step);
-    if (lane >= step) before += x;
-  }
-  __syncthreads();  // the sums have been read
-  if (lane == 31) control.sums[0][warp] = before;
-  __syncthreads();
-  int64_t total = 0;
-#pragma unroll
-  for (int w = 0; w <= kWarps; ++w) {
-    if (w < warp) before += control.sums[0][w];
-    total += control.sums[0][w];
-  }
-  before -= mine;
-  walk.position = share * blockIdx.x;
-  if (walk.position >= total) return;
-  walk.end = lmin(walk.position + share, total);
-  if (walk.position >= before && walk.position < before + mine) {
-    control.slot_start = before;
-    control.slot = mine0;
-  }
-  __syncthreads();
-  walk.slot_start = control.slot_start;
-  walk.slot = control.slot;
-
-  if (warp == kWarps) {
-    int stage = 0;
-    uint32_t phase = 0;
-    int64_t fed = 0;
-    bool failed = false;
-    for (int number = 0;; ++number) {
-      const bool more = walk.next(p, s);
-      if (!more) s.slot = -1;
-      const int at_segment = number & 1;
-      const bool taken = number < 2 || wait(shared_address(&control.taken[at_segment]), ((number >> 1) & 1) ^ 1, abort);
-      failed = __any_sync(0xffffffffu, !taken);
-      if (failed) break;
-      if (lane == 0) {
-        control.segments[at_segment] = s;
-        tc::arrive(shared_address(&control.posted[at_segment]));  // releases the segment
-      }
-      __syncwarp();
-      if (!more) break;
-      // The feeding warp: every tile of the stretch in order, through the ring.
-      const int32_t *entries = p.table + static_cast<int64_t>(s.slot) * p.table_stride;
-      for (int32_t first = s.tile0; first < s.tile1 && !failed; first += 32) {
-        // Lane i looks up the page(s) of tile first + i, and later issues its copies.
-        const int32_t row = (first + lane) * kTile;
-        const int parts = p.pages.page_size == 16 ? 2 : 1;
-        const int rows = parts == 1 ? kTile : 16;  // of a part
-        int copies = 0;                            // parts that the tile's visible rows lie in
-        const uint8_t *from[2][4];                 // 4-bit: key rows, key scales, value rows, value scales
-        int32_t y[2] = {0, 0};                     // 16-bit: the row among all pages'
-        if (first + lane < s.tile1) {
-          copies = parts == 1 || row + 16 >= s.seen_max ? 1 : 2;
-#pragma unroll
-          for (int part = 0; part < 2; ++part)
-            if (part < copies) {
-              int32_t page = entries[(row + part * 16) >> p.pages.page_shift];
-              if (page < 0 || page >= p.pages.pages) {
-                page = 0;
-                atomicOr(p.flag, kFlagRow);
-              }
-              const int64_t at = static_cast<int64_t>(page) * p.pages.page_size + (row & (p.pages.page_size - 1));
-              y[part] = static_cast<int32_t>(at);
-              from[part][0] = p.pages.keys + at * L::kRowBytes;
-              from[part][1] = reinterpret_cast<const uint8_t *>(p.pages.key_scales) + at * L::kScaleBytes;
-              from[part][2] = p.pages.values + at * L::kRowBytes;
-              from[part][3] = reinterpret_cast<const uint8_t *>(p.pages.value_scales) + at * L::kScaleBytes;
-            }
-        }
-        const int32_t here = min(32, s.tile1 - first);
-        for (int32_t j = 0; j < here; ++j) {
-          const uint32_t at = base + stage * L::kStage, barrier = full + stage * 8;
-          bool given_up = false;
-          if (lane == j) {
-            given_up = fed >= L::kStages && !wait(empty + stage * 8, phase ^ 1, abort);
-            if (!given_up) {
-              tc::expect_bytes(barrier, copies * rows * (L::kStage / kTile));
-#pragma unroll
-              for (int part = 0; part < 2; ++part)
-                if (part < copies)
-#pragma unroll
-                  for (int side = 0; side < 2; ++side) {
-                    const uint32_t to = at + side * (L::kCodes + L::kScales);
-                    if constexpr (GROUP == 0) {
-#pragma unroll
-                      for (int box = 0; box < D / 64; ++box)  // 64 channels wide
-                        tc::tma_box(to + box * (kTile * 128) + part * 16 * 128, side ? &value_map : &key_map, box * 64,
-                                    y[part], barrier);
-                    } else {
-                      bulk_copy(to + part * 16 * L::kRowBytes, from[part][2 * side], rows * L::kRowBytes, barrier);
-                      bulk_copy(to + L::kCodes + part * 16 * L::kScaleBytes, from[part][2 * side + 1],
-                                rows * L::kScaleBytes, barrier);
-                    }
-                  }
-            }
-          }
-          // The warp stays together: a lane that ran ahead would find an older
-          // phase of its stage's barrier with the parity that it waits for.
-          failed = __any_sync(0xffffffffu, given_up || *abort);
-          if (failed) break;
-          ++fed;
-          if (++stage == L::kStages) {
-            stage = 0;
-            phase ^= 1;
-          }
-        }
-      }
-      if (failed) break;
+    if (lane == 0) {
+      control.sums[0][warp] = tiles_sum;
+      control.sums[1][warp] = units_sum;
     }
-    // Given up: leave only after the copies in flight have landed.
-    if (failed) {
-      if (lane == 0) atomicOr(p.flag, kFlagTimeout);
-      for (int64_t n = fed > L::kStages ? fed - L::kStages : 0; n < fed; ++n)
-        tc::wait_phase(full + static_cast<int>(n % L::kStages) * 8, static_cast<uint32_t>(n / L::kStages) & 1, nullptr);
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < L::kStages; ++i) tc::init_barrier(shared_address(&control.landed[i]), 1);
+      asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+      *abort = 0;
     }
-    return;
+    __syncthreads();
+    tiles_sum = units_sum = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      tiles_sum += control.sums[0][w];
+      units_sum += control.sums[1][w];
+    }
+    // With few units a block takes a piece of one unit (a unit rounded up to
+    // whole pieces): sum ceil(tiles / share) <= tiles_sum / share + units <=
+    // grid.  A second unit costs a block its start and its end once more, some
+    // 4 us; rounding costs the blocks units / grid of their time.  So with many
+    // units the shares are equal and cross the units' ends.
+    const bool pieces_apart = units_sum * 4 <= gridDim.x;
+    const int64_t blocks = pieces_apart ? gridDim.x - units_sum : gridDim.x;
+    share = lmax(divide(tiles_sum + blocks - 1, blocks), kMinTiles);
+    const int32_t round = pieces_apart ? static_cast<int32_t>(share) : 1;
+    int64_t mine = 0;
+    for (int32_t i = mine0; i < mine1; ++i) {
+      if (mine1 - mine0 > 1) slot_work<L::kRows>(p, i, s, units);
+      mine += units *
+              (pieces_apart ? static_cast<int64_t>((s.unit_tiles + round - 1) / round) * round : s.unit_tiles);
+    }
+    int64_t before = mine;
+#pragma unroll
+    for (int step = 1; step < 32; step <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, before, step);
+      if (lane >= step) before += x;
+    }
+    __syncthreads();  // the sums have been read
+    if (lane == 31) control.sums[0][warp] = before;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += control.sums[0][w];
+      total += control.sums[0][w];
+    }
+    before -= mine;
+    const int64_t start = share * blockIdx.x;
+    if (start >= total) return;
+    if (start >= before && start < before + mine) {
+      Walk<L::kRows> walk{start, lmin(start + share, total), before, mine0, round};
+      walk.next(p, s);
+      control.segments[0] = s;
+      control.walk = walk;
+    }
+    __syncthreads();
   }
 
   Consumer<T, D, GROUP, NT> c;
@@ -851,7 +735,7 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
   float *factors = reinterpret_cast<float *>(shared + L::kFactorAt);
   int32_t *seen_by = reinterpret_cast<int32_t *>(shared + L::kSeenAt);
   float *stat_top = reinterpret_cast<float *>(shared + L::kStatsAt), *stat_sum = stat_top + kWarps * L::kRows;
-  float *scratch = reinterpret_cast<float *>(shared + L::kScratchAt);
+  float *scratch = reinterpret_cast<float *>(shared);
   const uint8_t *query_at = shared + L::kQueryAt;
   const int g = lane >> 2, t = lane & 3;
   // A negative scale is taken by the queries, so that the largest score is the
@@ -859,20 +743,69 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
   const uint32_t turn = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
   constexpr float kLeastFactor = 1e-37f;
   int pieces = 0;
-  int stage = warp;  // of this warp's next tile
-  uint32_t phase = 0;
-  int turn_of = 0;   // the warp that the segment's first tile falls to
+  uint32_t phases = 0;  // of this warp's stages, a bit each
 
   for (int number = 0;; ++number) {
-    const int at_segment = number & 1;
-    const bool posted = wait(shared_address(&control.posted[at_segment]), (number >> 1) & 1, abort);
-    if (consumers_any(!posted)) {  // all warps go on or none
-      *abort = 1;
-      if (threadIdx.x == 0) atomicOr(p.flag, kFlagTimeout);
-      return;
-    }
-    const Segment &s = control.segments[at_segment];
+    const Segment &s = control.segments[number & 1];
     if (s.slot < 0) break;
+    // Warp w takes tiles w, w + kWarps, .. of the stretch, and moves them into
+    // its own stages.  Lane i knows the page(s) of its tile number 32 k + i.
+    const int32_t tile0 = s.tile0 + warp, seen_min = s.seen_min, seen_max = s.seen_max;
+    const int32_t own = max((s.tile1 - tile0 + kWarps - 1) / kWarps, 0);
+    int32_t page0 = 0, page1 = 0;
+    const auto look_up = [&](int32_t n) {
+      const int32_t *entries = p.table + static_cast<int64_t>(s.slot) * p.table_stride;
+      const int32_t row = (tile0 + (n + lane) * kWarps) * kTile;
+      if (n + lane < own) {
+        page0 = entries[row >> p.pages.page_shift];
+        if (p.pages.page_size == 16 && row + 16 < seen_max) page1 = entries[(row + 16) >> p.pages.page_shift];
+        if (static_cast<uint32_t>(page0) >= static_cast<uint32_t>(p.pages.pages) ||
+            static_cast<uint32_t>(page1) >= static_cast<uint32_t>(p.pages.pages)) {
+          page0 = page1 = 0;
+          atomicOr(p.flag, kFlagRow);
+        }
+      }
+    };
+    const auto feed = [&](int32_t n) {
+      if ((n & 31) == 0) look_up(n);
+      if (lane != (n & 31)) return;
+      const int slot = warp * L::kDepth + (L::kDepth == 2 ? n & 1 : 0);
+      const uint32_t to = base + slot * L::kStage, barrier = shared_address(&control.landed[slot]);
+      const int32_t row = (tile0 + n * kWarps) * kTile;
+      const bool halves = p.pages.page_size == 16;
+      const int rows = halves ? 16 : kTile;
+      const int copies = halves && row + 16 < seen_max ? 2 : 1;  // pages that the tile's visible rows lie in
+      tc::expect_bytes(barrier, copies * rows * (L::kStage / kTile));
+      for (int part = 0; part < copies; ++part) {
+        const int64_t y = static_cast<int64_t>(part ? page1 : page0) * p.pages.page_size +
+                          (row & (p.pages.page_size - 1));
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+          const uint32_t at = to + side * (L::kCodes + L::kScales);
+          if constexpr (GROUP == 0) {
+#pragma unroll
+            for (int box = 0; box < D / 64; ++box)  // 64 channels wide
+              tc::tma_box(at + box * (kTile * 128) + part * 16 * 128, side ? &value_map : &key_map, box * 64,
+                          static_cast<int>(y), barrier);
+          } else {
+            bulk_copy(at + part * 16 * L::kRowBytes, (side ? p.pages.values : p.pages.keys) + y * L::kRowBytes,
+                      rows * L::kRowBytes, barrier);
+            bulk_copy(at + L::kCodes + part * 16 * L::kScaleBytes,
+                      (side ? p.pages.value_scales : p.pages.key_scales) + y * L::kGroups, rows * L::kScaleBytes, barrier);
+          }
+        }
+      }
+    };
+    for (int32_t n = 0; n < min(own, L::kDepth); ++n) feed(n);
+    __syncwarp();
+    if (threadIdx.x == kThreads - 1) {  // a thread of the warp with the fewest tiles finds the next segment
+      Walk<L::kRows> walk = control.walk;
+      Segment next;
+      if (!walk.next(p, next)) next.slot = -1;
+      control.segments[(number + 1) & 1] = next;
+      control.walk = walk;
+    }
+    __syncwarp();
     const int32_t head = s.slot - s.sequence * p.heads;
     const int32_t rows_total = s.tokens * p.groups;
     // Query fragments: the B operand of a k-step holds, for query row g, the
@@ -938,7 +871,7 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
         if (column == 0) factors[row] = fmaxf(fabsf(p.scale_log2) * 0x1p20f * from_unit, kLeastFactor);
       }
     }
-    consumers_sync();
+    __syncthreads();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -946,29 +879,29 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
         c.factor[nt][i] = factors[nt * 8 + 2 * t + i];
       }
     c.clear();
-    const int32_t tile0 = s.tile0, tiles = max(s.tile1 - s.tile0, 0), seen_min = s.seen_min;
-    // The stretch's tiles go to the warps in turn.
-    for (int32_t i = (warp - turn_of) & (kWarps - 1); i < tiles; i += kWarps) {
-      uint8_t *const at = shared + stage * L::kStage;
-      const bool landed = wait(full + stage * 8, phase, abort);
-      const int32_t first_row = (tile0 + i) * kTile;
-      if (!landed) {  // every barrier below is still met
+    for (int32_t n = 0; n < own; ++n) {
+      const int slot = L::kDepth == 2 ? n & 1 : 0;
+      const uint32_t barrier = shared_address(&control.landed[warp * L::kDepth + slot]);
+      uint8_t *const at = shared + (warp * L::kDepth + slot) * L::kStage;
+      const int32_t first_row = (tile0 + n * kWarps) * kTile;
+      const bool landed = __all_sync(0xffffffffu, wait(barrier, (phases >> slot) & 1, abort));
+      if (!landed) {
+        // Given up: nothing more is computed, but every barrier is still met,
+        // and the copy in flight gets its time to land.
         if (lane == 0) atomicOr(p.flag, kFlagTimeout);
+        *abort = 1;
+        tc::wait_phase(barrier, (phases >> slot) & 1, nullptr);
       } else if (first_row + kTile > seen_min) {
-        c.template tile<true>(at, query_at, group_sums, lane, first_row, s.seen_max, seen_by);
+        c.template tile<true>(at, query_at, group_sums, lane, first_row, seen_max, seen_by);
         if constexpr (GROUP == 0) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       } else {
-        c.template tile<false>(at, query_at, group_sums, lane, first_row, s.seen_max, seen_by);
+        c.template tile<false>(at, query_at, group_sums, lane, first_row, seen_max, seen_by);
       }
+      phases ^= 1u << slot;
       __syncwarp();
-      if (lane == 0) tc::arrive(empty + stage * 8);
-      stage += kWarps;
-      if (stage >= L::kStages) {
-        stage -= L::kStages;
-        phase ^= 1;
-      }
+      if (n + L::kDepth < own) feed(n + L::kDepth);
+      __syncwarp();
     }
-    turn_of = (turn_of + tiles) & (kWarps - 1);
 
     // Join the warps.
 #pragma unroll
@@ -987,7 +920,7 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
           stat_sum[warp * L::kRows + nt * 8 + 2 * t + i] = c.sum[nt][i];
         }
       }
-    consumers_sync();
+    __syncthreads();  // the stages turn into scratch
     const bool whole_unit = s.starts && s.ends;
     float *partial = p.partials + (static_cast<int64_t>(blockIdx.x) * 2 + (s.starts ? 1 : 0)) * L::kRows * (D + 2);
 #pragma unroll
@@ -1020,7 +953,7 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
           }
         }
       }
-      consumers_sync();
+      __syncthreads();
       constexpr int kEach = D / 16;  // channels per thread: 16 threads a row
       const int row = threadIdx.x >> 4, channel = (threadIdx.x & 15) * kEach;
       float best = stat_top[nt * 8 + row];
@@ -1068,21 +1001,21 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
           }
         }
       }
-      consumers_sync();
+      __syncthreads();
     }
     if (!whole_unit) {
       if (threadIdx.x == 0) control.pending[pieces] = s;
       ++pieces;
     }
-    consumers_sync();
-    if (threadIdx.x == 0) tc::arrive(shared_address(&control.taken[at_segment]));
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the scratch turns into stages
+    __syncthreads();
   }
   if (pieces == 0) return;
 
   // A block has at most two units that it shares, the first and the last of its
   // stretch.  Their results are announced together at the end: one release,
   // and no wait in between.  The block that arrives last at a unit joins it.
-  consumers_sync();
+  __syncthreads();
   if (threadIdx.x < pieces) {
     const Segment &of = control.pending[threadIdx.x];
     const int64_t first = divide(of.unit_start, share), last = divide(of.unit_start + of.unit_tiles - 1, share);
@@ -1096,7 +1029,7 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
     if (joins) p.counters[first] = 0;  // as the next call expects it
     control.arrived[threadIdx.x] = joins;
   }
-  consumers_sync();
+  __syncthreads();
   for (int piece = 0; piece < pieces; ++piece) {
     if (!control.arrived[piece]) continue;
     const Segment &s = control.pending[piece];
@@ -1122,7 +1055,7 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
     }
     joined[threadIdx.x] = best;
     joined[kWarps * 32 + threadIdx.x] = weight_sum;
-    consumers_sync();
+    __syncthreads();
     best = -INFINITY, weight_sum = 0.0f;
     for (int i = own_row; i < kWarps * 32; i += L::kRows)
       add_part(best, weight_sum, joined[i], joined[kWarps * 32 + i]);
@@ -1131,7 +1064,7 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
       stat_sum[own_row] = weight_sum;
       if (own_row < rows_here) p.lse[out_row(p, s, s.row0 + own_row)] = natural(best, weight_sum);
     }
-    consumers_sync();
+    __syncthreads();
     // The outputs, four channels a thread at a time.
     for (int item = threadIdx.x; item < rows_here * (D / 4); item += kWarps * 32) {
       const int row = item / (D / 4), channel = item % (D / 4) * 4;
@@ -1154,7 +1087,7 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
       *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + out_row(p, s, s.row0 + row) * D + channel) =
           *reinterpret_cast<const uint2 *>(result);
     }
-    consumers_sync();  // before the next piece writes over the statistics
+    __syncthreads();  // before the next piece writes over the statistics
   }
 }
 
