@@ -2,7 +2,8 @@
 
 liblrk.so   <- csrc/host.cu, move.cu, score.cu, select.cu, fused.cu, project.cu, logits.cu,
                logits_tc.cu, scores_tc.cu, groups.cu,
-               arena.cu, plan.cu, paged_append.cu, paged_attention.cu (nvcc, sm_100a)
+               arena.cu, plan.cu, paged_append.cu, paged_attention.cu,
+               paged_attention_tc.cu (nvcc, sm_100a)
 _C          <- csrc/shim_C.cpp        (torch extension, links liblrk)
 _legacy_C   <- csrc/shim_legacy_C.cpp (torch extension, links liblrk)
 _host       <- csrc/shim_host.cpp     (pybind11 only, links liblrk)
@@ -49,6 +50,7 @@ CUDA_SOURCES = {
     "plan.cu": [],
     "paged_append.cu": [],
     "paged_attention.cu": [],
+    "paged_attention_tc.cu": [],
 }
 MODULES = {"_C": "shim_C.cpp", "_legacy_C": "shim_legacy_C.cpp", "_host": "shim_host.cpp"}
 EXT_SUFFIX = sysconfig.get_config_var("EXT_SUFFIX") or ".so"

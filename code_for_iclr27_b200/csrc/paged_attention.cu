@@ -28,19 +28,18 @@
 //   the subtraction of 8 sum f16(p scale_g) by one more matrix instruction per
 //   group with ones as A, so that it cancels exactly what was rounded.
 //
-// Split: the tiles of 32 rows of all slots, laid end to end, are divided
-// evenly over a persistent grid, so neither few slots nor ragged ones leave
-// SMs idle.  A slot whose tiles fall to several blocks leaves partial results
-// (maximum, sum, output) in the workspace; the block that arrives last joins
-// them in a fixed order, so the result does not depend on the arrival.
+// Tiles are 32 rows; how they are split over the blocks: paged_attention.cuh.
 #include <cuda.h>
 
 #include <algorithm>
 
-#include "paged.cuh"
-#include "tc.cuh"
+#include "paged_attention.cuh"
 
 namespace lrk {
+
+// Many query rows a slot (paged_attention_tc.cu).
+int launch_paged_attention_tc(const void *param, const lrk_pages &pages, int dtype, cudaStream_t stream);
+
 namespace {
 
 using namespace paged;
@@ -48,44 +47,8 @@ using namespace paged;
 constexpr int kTile = 32;   // rows per tile
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
+constexpr int kMatrixRows = 32;    // more query rows a slot than this: paged_attention_tc.cu
 constexpr int kMinTiles = kWarps;  // tiles per block, at least
-constexpr int kCounters = 4096;    // workspace: arrival counters, then partial results
-
-// Division by a number that the host knows: n / d for n below 2^31 as a
-// product (Granlund and Montgomery's round-up method).
-struct Divider {
-  uint32_t multiplier, shift;
-  static Divider of(uint32_t d) {
-    Divider r{0, 0};
-    while ((uint64_t{1} << r.shift) < d) ++r.shift;
-    r.multiplier = static_cast<uint32_t>(((((uint64_t{1} << r.shift) - d) << 32) / d) + 1);
-    return r;
-  }
-  __device__ __forceinline__ int32_t operator()(int32_t n) const {
-    return static_cast<int32_t>((__umulhi(static_cast<uint32_t>(n), multiplier) + static_cast<uint32_t>(n)) >> shift);
-  }
-};
-
-struct AttentionParam {
-  Pages pages;
-  const int32_t *table;
-  int64_t table_stride;
-  int32_t capacity;  // rows that a slot's table entries can hold
-  const int32_t *lengths;
-  const int32_t *token_starts;
-  int32_t slots, tokens;
-  const void *queries;
-  int64_t query_token, query_head;
-  int heads, groups;
-  Divider by_heads, by_groups;
-  float scale_log2;
-  bool causal;
-  void *out;
-  float *lse;
-  uint32_t *counters;
-  float *partials;
-  uint32_t *flag;
-};
 
 template <typename T, int D, int GROUP, int NT>
 struct Layout {
@@ -150,16 +113,6 @@ __device__ __forceinline__ uint32_t pack(const __nv_bfloat16 *, float lo, float 
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-__device__ __forceinline__ uint32_t shared_address(const void *p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 template <int WORDS>
 __device__ __forceinline__ void load_words(const uint8_t *from, uint32_t *w) {
   if constexpr (WORDS == 4) {
@@ -176,103 +129,12 @@ __device__ __forceinline__ float2 load_pair(const uint8_t *from) {  // (scale, o
   return __half22float2(*reinterpret_cast<const __half2 *>(from));
 }
 
-__device__ __forceinline__ void bulk_copy(uint32_t to, const void *from, uint32_t bytes, uint32_t barrier) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(to),
-               "l"(from), "r"(bytes), "r"(barrier)
-               : "memory");
-}
-
-__device__ __forceinline__ bool wait(uint32_t barrier, uint32_t parity, volatile int *abort) {
-  uint32_t done;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(done)
-      : "r"(barrier), "r"(parity)
-      : "memory");
-  return done || tc::wait_phase(barrier, parity, abort);
-}
-
-// a / b for a >= 0, b > 0.  Out of line: the 64-bit division is some hundred
-// instructions that hardly any call needs.
-__device__ __noinline__ int64_t divide_long(int64_t a, int64_t b) { return a / b; }
-__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
-  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
-  return divide_long(a, b);
-}
-
-// A stretch of one unit's tiles: a unit is a slot and a block of its query rows.
-struct Segment {
-  int64_t unit_start;                   // where the unit begins among all units' tiles
-  int32_t unit_tiles;
-  int32_t slot, sequence;
-  int32_t tokens, first_token;          // of the sequence
-  int32_t row0;                         // first query row (token * groups + head in group) of the unit
-  int32_t length;                       // of the slot
-  int32_t tile0, tile1;                 // tiles of the stretch, those beyond every query's rows left out
-  int32_t seen_max, seen_min;           // rows seen by the unit's last and first query
-  bool starts, ends;                    // the stretch holds the unit's first / last tile
-};
-
-static_assert(sizeof(Segment) <= 64, "the layout keeps 64 bytes for a segment");
-
-// What a slot asks for: tiles per unit (at least one, so that a query without
-// a visible row gets its zeros), and units.
-template <int ROWS>
-__device__ __forceinline__ void slot_work(const AttentionParam &p, int32_t slot, Segment &s, int32_t &units) {
-  s.slot = slot;
-  s.sequence = p.by_heads(slot);
-  s.first_token = min(max(p.token_starts[s.sequence], 0), p.tokens);
-  s.tokens = max(min(p.token_starts[s.sequence + 1], p.tokens) - s.first_token, 0);
-  s.length = min(max(p.lengths[slot], 0), p.capacity);
-  s.unit_tiles = max((s.length + kTile - 1) / kTile, 1);
-  units = (s.tokens * p.groups + ROWS - 1) / ROWS;
-}
-
-__device__ __forceinline__ int32_t rows_seen(const AttentionParam &p, const Segment &s, int32_t row) {
-  return p.causal ? max(s.length - s.tokens + p.by_groups(row) + 1, 0) : s.length;
-}
-
-// Walks a block's share of all units' tiles, laid end to end with every unit
-// rounded up to a multiple of `round` tiles.
-template <int ROWS>
-struct Walk {
-  int64_t position, end;
-  int64_t slot_start;
-  int32_t slot, round;
-
-  __device__ __forceinline__ bool next(const AttentionParam &p, Segment &s) {
-    if (position >= end) return false;
-    int64_t span;
-    for (;; ++slot) {
-      if (slot >= p.slots) return false;
-      int32_t units;
-      slot_work<ROWS>(p, slot, s, units);
-      span = round == 1 ? s.unit_tiles : static_cast<int64_t>((s.unit_tiles + round - 1) / round) * round;
-      if (position < slot_start + span * units) break;
-      slot_start += span * units;
-    }
-    const int64_t unit = divide(position - slot_start, span);
-    s.unit_start = slot_start + unit * span;
-    s.tile0 = static_cast<int32_t>(position - s.unit_start);
-    const int64_t stop = lmin(end, s.unit_start + span);
-    s.tile1 = min(static_cast<int32_t>(stop - s.unit_start), s.unit_tiles);
-    s.starts = s.tile0 == 0;
-    s.ends = s.tile1 == s.unit_tiles;
-    position = stop;
-    s.row0 = static_cast<int32_t>(unit * ROWS);
-    s.seen_min = rows_seen(p, s, s.row0);
-    s.seen_max = rows_seen(p, s, min(s.row0 + ROWS, s.tokens * p.groups) - 1);
-    s.tile1 = min(s.tile1, (s.seen_max + kTile - 1) / kTile);
-    return true;
-  }
-};
-
 // A block's shared words beside the stages.
 template <int ROWS>
 struct Control {
   uint64_t landed[2 * kWarps];  // barriers of the stages
   int64_t sums[2][kWarps];
-  Walk<ROWS> walk;
+  Walk<ROWS, kTile> walk;
   int32_t abort;
   int32_t arrived[2];
   Segment pending[2];
@@ -619,24 +481,6 @@ struct Consumer {
   }
 };
 
-// Adds a part's (maximum, sum) to another's.
-__device__ __forceinline__ void add_part(float &best, float &sum, float m, float l) {
-  const float next = max_nan(best, m);
-  sum = (best == -INFINITY ? 0.0f : sum * exp2_fast(best - next)) + (m == -INFINITY ? 0.0f : l * exp2_fast(m - next));
-  best = next;
-}
-
-// lse of weights exp2(s - top) that add up to sum.
-__device__ __noinline__ float natural(float top, float sum) {
-  return sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945f;
-}
-
-// The output row of a unit's query row.
-__device__ __forceinline__ int64_t out_row(const AttentionParam &p, const Segment &s, int32_t query_row) {
-  const int32_t token = p.by_groups(query_row), head = s.slot - s.sequence * p.heads;
-  return (static_cast<int64_t>(s.first_token + token) * p.heads + head) * p.groups + (query_row - token * p.groups);
-}
-
 template <typename T, int D, int GROUP, int NT>
 __global__ __launch_bounds__(kThreads, (Layout<T, D, GROUP, NT>::kBlocksPerSm))
 void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_constant__ CUtensorMap key_map,
@@ -653,82 +497,13 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
     return;
   }
 
-  // All slots' tiles and units, and from them the blocks' share.
-  const int32_t each = (p.slots + kThreads - 1) / kThreads;
-  const int32_t mine0 = min(static_cast<int32_t>(threadIdx.x) * each, p.slots), mine1 = min(mine0 + each, p.slots);
-  int64_t share;
-  {
-    Segment s;
-    int64_t tiles_sum = 0, units_sum = 0;
-    int32_t units = 0;
-    for (int32_t i = mine0; i < mine1; ++i) {
-      slot_work<L::kRows>(p, i, s, units);
-      units_sum += units;
-      tiles_sum += static_cast<int64_t>(units) * s.unit_tiles;
-      if (blockIdx.x == 0 && p.lengths[i] > p.capacity) atomicOr(p.flag, kFlagRow);
-    }
-#pragma unroll
-    for (int step = 16; step > 0; step >>= 1) {
-      tiles_sum += __shfl_xor_sync(0xffffffffu, tiles_sum, step);
-      units_sum += __shfl_xor_sync(0xffffffffu, units_sum, step);
-    }
-    if (lane == 0) {
-      control.sums[0][warp] = tiles_sum;
-      control.sums[1][warp] = units_sum;
-    }
-    if (threadIdx.x == 0) {
-      for (int i = 0; i < L::kStages; ++i) tc::init_barrier(shared_address(&control.landed[i]), 1);
-      asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-      *abort = 0;
-    }
-    __syncthreads();
-    tiles_sum = units_sum = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      tiles_sum += control.sums[0][w];
-      units_sum += control.sums[1][w];
-    }
-    // With few units a block takes a piece of one unit (a unit rounded up to
-    // whole pieces): sum ceil(tiles / share) <= tiles_sum / share + units <=
-    // grid.  A second unit costs a block its start and its end once more, some
-    // 4 us; rounding costs the blocks units / grid of their time.  So with many
-    // units the shares are equal and cross the units' ends.
-    const bool pieces_apart = units_sum * 4 <= gridDim.x;
-    const int64_t blocks = pieces_apart ? gridDim.x - units_sum : gridDim.x;
-    share = lmax(divide(tiles_sum + blocks - 1, blocks), kMinTiles);
-    const int32_t round = pieces_apart ? static_cast<int32_t>(share) : 1;
-    int64_t mine = 0;
-    for (int32_t i = mine0; i < mine1; ++i) {
-      if (mine1 - mine0 > 1) slot_work<L::kRows>(p, i, s, units);
-      mine += units *
-              (pieces_apart ? static_cast<int64_t>((s.unit_tiles + round - 1) / round) * round : s.unit_tiles);
-    }
-    int64_t before = mine;
-#pragma unroll
-    for (int step = 1; step < 32; step <<= 1) {
-      const int64_t x = __shfl_up_sync(0xffffffffu, before, step);
-      if (lane >= step) before += x;
-    }
-    __syncthreads();  // the sums have been read
-    if (lane == 31) control.sums[0][warp] = before;
-    __syncthreads();
-    int64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += control.sums[0][w];
-      total += control.sums[0][w];
-    }
-    before -= mine;
-    const int64_t start = share * blockIdx.x;
-    if (start >= total) return;
-    if (start >= before && start < before + mine) {
-      Walk<L::kRows> walk{start, lmin(start + share, total), before, mine0, round};
-      walk.next(p, s);
-      control.segments[0] = s;
-      control.walk = walk;
-    }
-    __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::kStages; ++i) tc::init_barrier(shared_address(&control.landed[i]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    *abort = 0;
   }
+  int64_t share;
+  if (!begin<kThreads, kMinTiles>(p, &control.sums[0][0], share, control.walk, control.segments[0])) return;
 
   Consumer<T, D, GROUP, NT> c;
   float *group_sums = reinterpret_cast<float *>(shared + L::kSumsAt);
@@ -799,7 +574,7 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
     for (int32_t n = 0; n < min(own, L::kDepth); ++n) feed(n);
     __syncwarp();
     if (threadIdx.x == kThreads - 1) {  // a thread of the warp with the fewest tiles finds the next segment
-      Walk<L::kRows> walk = control.walk;
+      Walk<L::kRows, kTile> walk = control.walk;
       Segment next;
       if (!walk.next(p, next)) next.slot = -1;
       control.segments[(number + 1) & 1] = next;
@@ -1012,83 +787,8 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
   }
   if (pieces == 0) return;
 
-  // A block has at most two units that it shares, the first and the last of its
-  // stretch.  Their results are announced together at the end: one release,
-  // and no wait in between.  The block that arrives last at a unit joins it.
-  __syncthreads();
-  if (threadIdx.x < pieces) {
-    const Segment &of = control.pending[threadIdx.x];
-    const int64_t first = divide(of.unit_start, share), last = divide(of.unit_start + of.unit_tiles - 1, share);
-    uint32_t before_me;
-    // Releases this block's results (after the barrier) and acquires the others'.
-    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
-                 : "=r"(before_me)
-                 : "l"(p.counters + first)
-                 : "memory");
-    const bool joins = before_me == static_cast<uint32_t>(last - first);
-    if (joins) p.counters[first] = 0;  // as the next call expects it
-    control.arrived[threadIdx.x] = joins;
-  }
-  __syncthreads();
-  for (int piece = 0; piece < pieces; ++piece) {
-    if (!control.arrived[piece]) continue;
-    const Segment &s = control.pending[piece];
-    const int64_t first = divide(s.unit_start, share), last = divide(s.unit_start + s.unit_tiles - 1, share);
-    const int32_t parts = static_cast<int32_t>(last - first) + 1;
-    const int32_t rows_here = min(L::kRows, s.tokens * p.groups - s.row0);
-    constexpr int64_t kPart = L::kRows * (D + 2);
-    // Part 0 is the first block's second result, part i > 0 the first result of
-    // block first + i.
-    const float *from = p.partials + (first * 2) * kPart;
-    auto part_at = [&](int32_t i) { return from + (2 * static_cast<int64_t>(i) + (i == 0 ? 1 : 0)) * kPart; };
-    // Maxima and sums: thread (row, every kAcrossth part), joined over shared memory.
-    constexpr int kApart = kWarps * 32 / L::kRows;
-    constexpr int kHeld = (kWarps * 8 * L::kPitch - 2 * kWarps * 32) / L::kRows;  // parts whose maxima are kept
-    float *joined = scratch + kHeld * L::kRows;
-    const int own_row = threadIdx.x % L::kRows;
-    float best = -INFINITY, weight_sum = 0.0f;
-#pragma unroll 4
-    for (int32_t i = threadIdx.x / L::kRows; i < parts; i += kApart) {
-      const float m = __ldcg(part_at(i) + L::kRows * D + own_row), l = __ldcg(part_at(i) + L::kRows * (D + 1) + own_row);
-      if (i < kHeld) scratch[i * L::kRows + own_row] = m;
-      add_part(best, weight_sum, m, l);
-    }
-    joined[threadIdx.x] = best;
-    joined[kWarps * 32 + threadIdx.x] = weight_sum;
-    __syncthreads();
-    best = -INFINITY, weight_sum = 0.0f;
-    for (int i = own_row; i < kWarps * 32; i += L::kRows)
-      add_part(best, weight_sum, joined[i], joined[kWarps * 32 + i]);
-    if (threadIdx.x < L::kRows) {
-      stat_top[own_row] = best;
-      stat_sum[own_row] = weight_sum;
-      if (own_row < rows_here) p.lse[out_row(p, s, s.row0 + own_row)] = natural(best, weight_sum);
-    }
-    __syncthreads();
-    // The outputs, four channels a thread at a time.
-    for (int item = threadIdx.x; item < rows_here * (D / 4); item += kWarps * 32) {
-      const int row = item / (D / 4), channel = item % (D / 4) * 4;
-      const float top = stat_top[row];
-      float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-      for (int32_t i = 0; i < parts; ++i) {
-        const float *part = part_at(i);
-        const float4 x = __ldcg(reinterpret_cast<const float4 *>(part + row * D + channel));
-        const float m = i < kHeld ? scratch[i * L::kRows + row] : __ldcg(part + L::kRows * D + row);
-        const float w = m == -INFINITY ? 0.0f : exp2_fast(m - top);
-        value.x = fmaf(w, x.x, value.x);
-        value.y = fmaf(w, x.y, value.y);
-        value.z = fmaf(w, x.z, value.z);
-        value.w = fmaf(w, x.w, value.w);
-      }
-      const float inverse = stat_sum[row] == 0.0f ? 0.0f : 1.0f / stat_sum[row];
-      __align__(8) const T result[4] = {from_float<T>(value.x * inverse), from_float<T>(value.y * inverse),
-                                        from_float<T>(value.z * inverse), from_float<T>(value.w * inverse)};
-      *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + out_row(p, s, s.row0 + row) * D + channel) =
-          *reinterpret_cast<const uint2 *>(result);
-    }
-    __syncthreads();  // before the next piece writes over the statistics
-  }
+  join<T, D, L::kRows, kThreads>(p, control.pending, control.arrived, pieces, share, scratch, kWarps * 8 * L::kPitch,
+                                 stat_top, stat_sum);
 }
 
 template <typename T, int D, int GROUP, int NT>
@@ -1195,6 +895,7 @@ extern "C" int lrk_paged_attention(const lrk_pages *pages, const int32_t *table,
   p.counters = static_cast<uint32_t *>(workspace);
   p.partials = reinterpret_cast<float *>(p.counters + kCounters);
   p.flag = flag;
+  if (ceil_div(tokens, sequences) * p.groups > kMatrixRows) return launch_paged_attention_tc(&p, *pages, dtype, stream);
   if (dtype == LRK_F16)
     return pages->dimension == 64 ? launch_attention<__half, 64>(p, *pages, tokens, sequences, stream)
                                   : launch_attention<__half, 128>(p, *pages, tokens, sequences, stream);
