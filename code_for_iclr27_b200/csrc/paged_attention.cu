@@ -49,6 +49,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMatrixRows = 32;    // more query rows a slot than this: paged_attention_tc.cu
 constexpr int kMinTiles = kWarps;  // tiles per block, at least
+constexpr int kCrossing = 10;      // a second unit's cost in tiles: its start, its end, its join
 
 template <typename T, int D, int GROUP, int NT>
 struct Layout {
@@ -503,7 +504,7 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
     *abort = 0;
   }
   int64_t share;
-  if (!begin<kThreads, kMinTiles>(p, &control.sums[0][0], share, control.walk, control.segments[0])) return;
+  if (!begin<kThreads, kMinTiles, kCrossing>(p, &control.sums[0][0], share, control.walk, control.segments[0])) return;
 
   Consumer<T, D, GROUP, NT> c;
   float *group_sums = reinterpret_cast<float *>(shared + L::kSumsAt);

@@ -71,14 +71,20 @@ __device__ __forceinline__ void bulk_copy(uint32_t to, const void *from, uint32_
                : "memory");
 }
 
+__device__ __noinline__ bool wait_long(uint32_t barrier, uint32_t parity, volatile int *abort) {
+  return tc::wait_phase(barrier, parity, abort);
+}
+// Bounded wait for an mbarrier phase; the clock is read only after some tries.
 __device__ __forceinline__ bool wait(uint32_t barrier, uint32_t parity, volatile int *abort) {
-  uint32_t done;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(done)
-      : "r"(barrier), "r"(parity)
-      : "memory");
-  return done || tc::wait_phase(barrier, parity, abort);
+  uint32_t done = 0;
+#pragma unroll 1
+  for (int i = 0; i < 64 && !done; ++i)
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(barrier), "r"(parity)
+        : "memory");
+  return done || wait_long(barrier, parity, abort);
 }
 
 // a / b for a >= 0, b > 0.  Out of line: the 64-bit division is some hundred
@@ -158,7 +164,7 @@ struct Walk {
 
 // A block's share of the work and its first segment; false for a block without
 // any.  sums: 2 x THREADS / 32 shared words.  Ends with a barrier.
-template <int THREADS, int MIN_TILES, int ROWS, int TILE>
+template <int THREADS, int MIN_TILES, int CROSSING, int ROWS, int TILE>
 __device__ __forceinline__ bool begin(const AttentionParam &p, int64_t *sums, int64_t &share,
                                       Walk<ROWS, TILE> &of_block, Segment &segment) {
   constexpr int kWarps = THREADS / 32;
@@ -190,14 +196,16 @@ __device__ __forceinline__ bool begin(const AttentionParam &p, int64_t *sums, in
     tiles_sum += sums[w];
     units_sum += sums[kWarps + w];
   }
-  // With few units a block takes a piece of one unit (a unit rounded up to
-  // whole pieces): sum ceil(tiles / share) <= tiles_sum / share + units <=
-  // grid.  A second unit costs a block its start and its end once more, some
-  // 4 us; rounding costs the blocks units / grid of their time.  So with many
-  // units the shares are equal and cross the units' ends.
-  const bool pieces_apart = units_sum * 4 <= gridDim.x;
-  const int64_t blocks = pieces_apart ? gridDim.x - units_sum : gridDim.x;
-  share = lmax(divide(tiles_sum + blocks - 1, blocks), MIN_TILES);
+  // Shares are equal and cross the units' ends, or, where that costs at most
+  // CROSSING tiles more a block, every block takes a piece of one unit alone (a
+  // unit rounded up to whole pieces: sum ceil(tiles / share) <= tiles_sum /
+  // share + units <= grid).  CROSSING is what a second unit costs a block (its
+  // queries, its end, its join: some 4 us) in tiles.
+  const int64_t even = lmax(divide(tiles_sum + gridDim.x - 1, gridDim.x), MIN_TILES);
+  const int64_t left = static_cast<int64_t>(gridDim.x) - units_sum;
+  const int64_t apart = left > 0 ? lmax(divide(tiles_sum + left - 1, left), MIN_TILES) : 0;
+  const bool pieces_apart = left > 0 && apart <= even + CROSSING;
+  share = pieces_apart ? apart : even;
   const int32_t round = pieces_apart ? static_cast<int32_t>(share) : 1;
   int64_t mine = 0;
   for (int32_t i = mine0; i < mine1; ++i) {

@@ -32,7 +32,8 @@ namespace {
 constexpr int kBlockThreads = 256;
 constexpr int kBlockRows = 128;
 constexpr int kBlocksOfSm = 2;
-constexpr int kLeastTiles = 4;
+constexpr int kLeastTiles = 2;    // tiles per block, at least
+constexpr int kUnitCrossing = 1;  // a second unit's cost in tiles, at 3 us a tile
 constexpr uint32_t kColumns = 256;  // of tensor memory
 
 template <typename T, int D, int GROUP>
@@ -122,6 +123,15 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return d;
 }
 
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 d, a, b;\n"
+      " mov.b64 {%0, %1}, d;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 __device__ __forceinline__ uint32_t pack2(const __half *, float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t *>(&h);
@@ -183,7 +193,7 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
     *abort = 0;
   }
   int64_t share;
-  if (!begin<kBlockThreads, kLeastTiles>(p, &control.sums[0][0], share, control.walk, control.segment)) return;
+  if (!begin<kBlockThreads, kLeastTiles, kUnitCrossing>(p, &control.sums[0][0], share, control.walk, control.segment)) return;
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(
                      shared_address(&control.columns)),
@@ -363,10 +373,10 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
           const __half2 pair = __hmul2(
               reinterpret_cast<const __half2 *>(value_stage + L::kCodes)[r * L::kGroups + c * 8 / GROUP], two_halves);
           const __half2 scale = __low2half2(pair), offset = __high2half2(pair);
-          // Rows beyond every query's may hold anything, and 0 NaN is NaN.
-          const bool none = first_row + r >= s.seen_max;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) n[k] = none ? __float2half2_rn(0.0f) : __hfma2(n[k], scale, offset);
+          for (int k = 0; k < 4; ++k) n[k] = __hfma2(n[k], scale, offset);
+          // Rows beyond every query's may hold anything, and 0 NaN is NaN.
+          if (first_row + r >= s.seen_max) n[0] = n[1] = n[2] = n[3] = __float2half2_rn(0.0f);
           *reinterpret_cast<uint4 *>(operands + L::kOperand + chunk_at(r, c, L::kTile)) = *reinterpret_cast<uint4 *>(n);
         }
       } else {
@@ -459,13 +469,15 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
       }
       const float shift = top == -INFINITY ? 0.0f : -top;
       uint32_t weights[L::kHalf / 2];
+      float2 both = make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int k = 0; k < L::kHalf / 2; ++k) {
         const float2 e = fma2(x[k], make_float2(factor, factor), make_float2(shift, shift));
         const float a = exp2_fast(e.x), b = exp2_fast(e.y);
-        sum += a + b;
+        both = add2(both, make_float2(a, b));
         weights[k] = pack2(static_cast<const W *>(nullptr), a, b);
       }
+      sum += both.x + both.y;
       const uint32_t weights_at = lanes + L::kScoreColumn + half * (L::kHalf / 2);
       if constexpr (L::kHalf == 32) tc::tmem_store16(weights_at, weights);
       else tmem_store8(weights_at, weights);
