@@ -23,6 +23,7 @@ namespace {
 using namespace paged;
 
 constexpr int kThreads = 128;
+constexpr int kManyTokens = 1024;  // from here on append_kernel goes BY_TOKENS
 
 struct AppendParam {
   Pages pages;
@@ -55,48 +56,70 @@ __device__ __forceinline__ int64_t find_sequence(const AppendParam &p, int64_t t
   return lo;
 }
 
-// x[0..15]: the rotated channels [first, first + 16) of a row.
-template <typename T>
-__device__ __forceinline__ void rotate16(const AppendParam &p, const T *row, const float *turn, int first, float *x) {
-  const int half = p.rotary_dim >> 1;
+// Eight floats from 16-byte aligned memory, four from as many.
+__device__ __forceinline__ void load_floats(const float *from, float *x) {
+  const float4 v = *reinterpret_cast<const float4 *>(from);
+  x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+}
+
+// A lane's 16 channels' rotation: x' = x cosine + other sine, where `other` is
+// the pair's other channel and the sine carries the sign.
+struct Turn {
+  float cosine[16], sine[16];
+  bool turns[2];  // whether the first and the last 8 channels are rotated
+};
+
+__device__ __forceinline__ void load_turn(const AppendParam &p, const float *table, int first, Turn &turn) {
+  const int pairs = p.rotary_dim >> 1;
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
     const int c = first + 8 * part;
-    float *y = x + 8 * part;
-    if (turn == nullptr || c >= p.rotary_dim) continue;
+    float *cosine = turn.cosine + 8 * part, *sine = turn.sine + 8 * part;
+    turn.turns[part] = table != nullptr && c < p.rotary_dim;
+    if (!turn.turns[part]) continue;
     if (p.interleaved) {
+      float a[4], b[4];
+      load_floats(table + (c >> 1), a);
+      load_floats(table + pairs + (c >> 1), b);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float cosine = turn[(c >> 1) + i], sine = turn[half + (c >> 1) + i];
-        const float a = y[2 * i], b = y[2 * i + 1];
-        y[2 * i] = __fsub_rn(__fmul_rn(a, cosine), __fmul_rn(b, sine));
-        y[2 * i + 1] = __fadd_rn(__fmul_rn(b, cosine), __fmul_rn(a, sine));
+        cosine[2 * i] = cosine[2 * i + 1] = a[i];
+        sine[2 * i] = -b[i];
+        sine[2 * i + 1] = b[i];
       }
-      continue;
-    }
-    const bool low = c < half;
-    const int at = low ? c : c - half;
-    float other[8];
-    load8(row + (low ? c + half : at), other);
+    } else {
+      const bool low = c < pairs;
+      const int at = low ? c : c - pairs;
+      load_floats(table + at, cosine);
+      load_floats(table + at + 4, cosine + 4);
+      load_floats(table + pairs + at, sine);
+      load_floats(table + pairs + at + 4, sine + 4);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float own = __fmul_rn(y[i], turn[at + i]), cross = __fmul_rn(other[i], turn[half + at + i]);
-      y[i] = low ? __fsub_rn(own, cross) : __fadd_rn(own, cross);
+      for (int i = 0; i < 8; ++i) sine[i] = low ? -sine[i] : sine[i];
     }
   }
 }
 
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4 &raw, float *x) {
+  const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = to_float<T>(e[i]);
+}
+
 // Quantises 16 channels per lane; the group / 16 lanes of a group are
 // neighbours.  Stores the lane's 8 bytes of codes and, once per group, the
-// scale and offset.
+// scale and offset; a negative row stores nothing.
 template <int D, int GROUP>
 __device__ __forceinline__ void store_codes(uint8_t *codes, __half2 *scales, int64_t row, int lane, const float *x) {
-  float lo = x[0], hi = x[0];
+  float lo = min_nan(x[0], x[1], x[2]), hi = max_nan(x[0], x[1], x[2]);
 #pragma unroll
-  for (int i = 1; i < 16; ++i) {
-    lo = min_nan(lo, x[i]);
-    hi = max_nan(hi, x[i]);
+  for (int i = 3; i < 15; i += 2) {
+    lo = min_nan(lo, x[i], x[i + 1]);
+    hi = max_nan(hi, x[i], x[i + 1]);
   }
+  lo = min_nan(lo, x[15]);
+  hi = max_nan(hi, x[15]);
 #pragma unroll
   for (int step = 1; step < GROUP / 16; step <<= 1) {
     lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, step));
@@ -108,12 +131,20 @@ __device__ __forceinline__ void store_codes(uint8_t *codes, __half2 *scales, int
   const bool fine = !__hisinf(scale) && !__hisnan(scale) && !__hisinf(offset) && !__hisnan(offset);
   const float inverse = step > 0.0f ? __frcp_rn(step) : 0.0f;
   const float centre = __half2float(offset);
+  // Held to [-8, 7] and added to 1.5 * 2^23 + 8, a level leaves its code, rounded
+  // to nearest even, in the sum's last bits; a word is sum code_i 16^i.
+  constexpr float kMagic = 12582920.0f;
+  constexpr uint32_t kMagicBits = 0x4B400000u;  // of 1.5 * 2^23
   uint32_t word[2] = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float level = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[i], centre), inverse)) + 8.0f, 0.0f), 15.0f);
-    word[i >> 3] |= static_cast<uint32_t>(level) << (4 * (i & 7));
-  }
+  for (int i = 7; i >= 0; --i)
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const float level = __fmul_rn(__fsub_rn(x[8 * w + i], centre), inverse);
+      word[w] = word[w] * 16 + __float_as_uint(__fadd_rn(fminf(fmaxf(level, -8.0f), 7.0f), kMagic));
+    }
+#pragma unroll
+  for (int w = 0; w < 2; ++w) word[w] -= kMagicBits * 0x11111111u;
   if (!fine) {
     word[0] = word[1] = 0;
     scale = offset = __ushort_as_half(0x7fff);
@@ -123,69 +154,120 @@ __device__ __forceinline__ void store_codes(uint8_t *codes, __half2 *scales, int
   if (lane % (GROUP / 16) == 0) scales[row * (D / GROUP) + lane / (GROUP / 16)] = __halves2half2(scale, offset);
 }
 
-// D / 16 neighbouring lanes per (token, row of keys, values or queries), 16
-// channels each; rows of a token are consecutive work items, so a warp reads
-// consecutive rows of the projection's output.
-template <typename T, int D, int GROUP>
+// D / 16 neighbouring lanes take a row of keys, values or queries, 16 channels
+// each.  BY_TOKENS: a block takes as many tokens as it has such lane groups and
+// four rows (heads) of each, so that a token's cosines and sines are read once,
+// all four rows are in flight at a time, and a head's appended rows are written
+// side by side.  Otherwise (few tokens) a block takes one token's rows.
+template <typename T, int D, int GROUP, bool BY_TOKENS>
 __global__ __launch_bounds__(kThreads) void append_kernel(const AppendParam p) {
-  constexpr int kLanes = D / 16;
-  const int lane = threadIdx.x % kLanes;
-  const int rows_per_token = 2 * p.heads + p.query_heads;
-  const int64_t items = p.tokens * rows_per_token;
-  const int64_t item = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / kLanes;
-  const bool live = item < items;
-  const int64_t token = live ? item / rows_per_token : 0;
-  const int part = live ? static_cast<int>(item % rows_per_token) : 0;
-  const bool is_key = part < p.heads, is_value = !is_key && part < 2 * p.heads;
+  constexpr int kLanes = D / 16, kTeams = kThreads / kLanes;
+  constexpr int kRows = BY_TOKENS ? 4 : 1;
+  const int lane = threadIdx.x % kLanes, team = threadIdx.x / kLanes, first = lane * 16;
+  const int parts = 2 * p.heads + p.query_heads;
+  // Blocks of the same tokens follow one another, so that the rows read (and
+  // the queries written) at a time lie together.
+  const uint32_t chunks = (parts + (BY_TOKENS ? kRows : kTeams) - 1) / (BY_TOKENS ? kRows : kTeams);
+  const uint32_t number = blockIdx.x / chunks, chunk = blockIdx.x - number * chunks;
+  const int64_t wanted = BY_TOKENS ? static_cast<int64_t>(number) * kTeams + team : number;
+  const int part0 = BY_TOKENS ? chunk * kRows : chunk * kTeams + team;
+  const bool live = wanted < p.tokens;
+  const int64_t token = live ? wanted : 0;
+  const int half = p.rotary_dim >> 1;
+
+  uint4 raw[kRows][2], pair[kRows][2];
+  int64_t place[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const int part = min(part0 + r, parts - 1);
+    const bool is_value = part >= p.heads && part < 2 * p.heads;
+    const T *from = part < p.heads ? static_cast<const T *>(p.keys) + token * p.key_token + part * p.key_head
+                    : is_value ? static_cast<const T *>(p.values) + token * p.value_token + (part - p.heads) * p.value_head
+                               : static_cast<const T *>(p.queries) + token * p.query_token +
+                                     (part - 2 * p.heads) * p.query_head;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int c = first + 8 * k;
+      raw[r][k] = *reinterpret_cast<const uint4 *>(from + c);
+      if (!is_value && !p.interleaved && c < p.rotary_dim)
+        pair[r][k] = *reinterpret_cast<const uint4 *>(from + (c < half ? c + half : c - half));
+    }
+  }
   const int64_t position = p.positions[token];
-  const float *turn = nullptr;
-  bool skip = !live;
-  if (p.rotary_dim > 0 && !is_value) {
-    if (position >= 0 && position < p.rotary_positions) turn = p.rotary + position * p.rotary_dim;
-    else skip = true;
-    if (skip && live && lane == 0) atomicOr(p.flag, kFlagPosition);
+  bool turned = p.rotary_dim > 0, lost = false;  // lost: a position outside the table
+  if (turned && (position < 0 || position >= p.rotary_positions)) {
+    turned = false;
+    lost = true;
   }
-  const T *from;
-  int64_t row = -1;
-  if (is_key || is_value) {
-    const int head = is_key ? part : part - p.heads;
-    from = is_key ? static_cast<const T *>(p.keys) + token * p.key_token + head * p.key_head
-                  : static_cast<const T *>(p.values) + token * p.value_token + head * p.value_head;
+  Turn turn;
+  load_turn(p, turned ? p.rotary + position * p.rotary_dim : nullptr, first, turn);
+  if (part0 < 2 * p.heads) {
     const int64_t sequence = find_sequence(p, token);
-    const int64_t first = p.token_starts[sequence], count = p.token_starts[sequence + 1] - first;
-    const int64_t slot = sequence * p.heads + head;
-    if (token >= first && token - first < count)
-      row = pool_row(p.pages, p.table, p.table_stride, p.table_width, slot, p.lengths[slot] - count + (token - first));
-    if (row < 0 && live && lane == 0) atomicOr(p.flag, kFlagRow);
-  } else {
-    from = static_cast<const T *>(p.queries) + token * p.query_token + (part - 2 * p.heads) * p.query_head;
+    const int64_t start = p.token_starts[sequence], count = p.token_starts[sequence + 1] - start;
+    const bool known = live && token >= start && token - start < count;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const int part = part0 + r;
+      place[r] = -1;
+      if (part >= 2 * p.heads) continue;
+      const int64_t slot = sequence * p.heads + (part < p.heads ? part : part - p.heads);
+      if (known)
+        place[r] = pool_row(p.pages, p.table, p.table_stride, p.table_width, slot,
+                            p.lengths[slot] - count + (token - start));
+      if (place[r] < 0 && live && lane == 0) atomicOr(p.flag, kFlagRow);
+      if (lost && part < p.heads) place[r] = -1;
+    }
   }
-  float x[16];
-  load8(from + lane * 16, x);
-  load8(from + lane * 16 + 8, x + 8);
-  if (!is_value) rotate16<T>(p, from, turn, lane * 16, x);
-  if (is_key || is_value) {
-    if (skip) row = -1;
-    uint8_t *pool = is_key ? p.pages.keys : p.pages.values;
-    if constexpr (GROUP == 0) {
-      if (row >= 0) {
-        T *to = reinterpret_cast<T *>(pool) + row * D + lane * 16;
-        store8(to, x);
-        store8(to + 8, x + 8);
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const int part = part0 + r;
+    if (BY_TOKENS && part >= parts) break;  // the same for the whole block
+    const bool is_key = part < p.heads, is_value = !is_key && part < 2 * p.heads;
+    float x[16];
+    unpack8<T>(raw[r][0], x);
+    unpack8<T>(raw[r][1], x + 8);
+    if (!is_value) {
+      if (lost && live && lane == 0 && part < parts) atomicOr(p.flag, kFlagPosition);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (!turn.turns[k]) continue;
+        float other[8], *own = x + 8 * k;
+        if (p.interleaved) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) other[i] = own[i ^ 1];
+        } else {
+          unpack8<T>(pair[r][k], other);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          own[i] = __fadd_rn(__fmul_rn(own[i], turn.cosine[8 * k + i]), __fmul_rn(other[i], turn.sine[8 * k + i]));
       }
     }
-    if (is_key && row >= 0 && lane == 0) p.pages.positions[row] = static_cast<float>(position);
-  } else if (!skip) {
-    T *to = static_cast<T *>(p.out_queries) + (token * p.query_heads + (part - 2 * p.heads)) * D + lane * 16;
-    store8(to, x);
-    store8(to + 8, x + 8);
-  }
-  if constexpr (GROUP != 0) {
-    // Every lane of the warp takes part in the group's shuffles; rows of
-    // queries, and rows without a place, store nothing.
-    const bool key_row = is_key || !is_value;
-    store_codes<D, GROUP>(key_row ? p.pages.keys : p.pages.values, key_row ? p.pages.key_scales : p.pages.value_scales,
-                          is_key || is_value ? row : -1, lane, x);
+    if (is_key || is_value) {
+      const int64_t row = place[r];
+      uint8_t *pool = is_key ? p.pages.keys : p.pages.values;
+      if constexpr (GROUP == 0) {
+        if (row >= 0) {
+          T *to = reinterpret_cast<T *>(pool) + row * D + first;
+          store8(to, x);
+          store8(to + 8, x + 8);
+        }
+      } else if constexpr (BY_TOKENS) {
+        store_codes<D, GROUP>(pool, is_key ? p.pages.key_scales : p.pages.value_scales, row, lane, x);
+      }
+      if (is_key && row >= 0 && lane == 0) p.pages.positions[row] = static_cast<float>(position);
+    } else if (live && !lost && part < parts) {
+      T *to = static_cast<T *>(p.out_queries) + (token * p.query_heads + (part - 2 * p.heads)) * D + first;
+      store8(to, x);
+      store8(to + 8, x + 8);
+    }
+    if constexpr (GROUP != 0 && !BY_TOKENS) {
+      // The warp's rows differ, and every lane takes part in the groups'
+      // shuffles: rows of queries, and rows without a place, store nothing.
+      store_codes<D, GROUP>(is_value ? p.pages.values : p.pages.keys,
+                            is_value ? p.pages.value_scales : p.pages.key_scales,
+                            part < 2 * p.heads ? place[r] : -1, lane, x);
+    }
   }
 }
 
@@ -201,60 +283,105 @@ struct ReadParam {
   uint32_t *flag;
 };
 
-// D / 16 lanes per row, keys and values of the row together.
+constexpr int kReadRows = 2;
+
+// D / 16 lanes per row, keys and values of the row together; a lane group takes
+// two neighbouring rows, which mostly share their slot's lookup.
 template <typename T, int D, int GROUP, typename S>
 __global__ __launch_bounds__(kThreads) void read_kernel(const ReadParam p) {
-  constexpr int kLanes = D / 16;
+  constexpr int kLanes = D / 16, kTeams = kThreads / kLanes;
   const int lane = threadIdx.x % kLanes;
-  const int64_t out_row = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / kLanes;
-  if (out_row >= p.rows) return;
-  int64_t lo = 0, hi = p.slots;
-  while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (p.row_starts[mid] <= out_row) lo = mid; else hi = mid;
+  const int64_t row0 = (static_cast<int64_t>(blockIdx.x) * kTeams + threadIdx.x / kLanes) * kReadRows;
+  if (row0 >= p.rows) return;
+  int64_t slot = 0;  // the last slot whose start is <= row0
+  for (int64_t hi = p.slots; hi - slot > 1;) {
+    const int64_t mid = (slot + hi) >> 1;
+    if (p.row_starts[mid] <= row0) slot = mid; else hi = mid;
   }
-  const int64_t place = out_row - p.row_starts[lo];
-  const int64_t row = place >= 0 && out_row < p.row_starts[lo + 1]
-                          ? pool_row(p.pages, p.table, p.table_stride, p.table_width, lo, p.first_rows[lo] + place)
-                          : -1;
-  if (row < 0) {
-    if (lane == 0) atomicOr(p.flag, kFlagRow);
-    return;
+  int64_t rows[kReadRows];
+#pragma unroll
+  for (int k = 0; k < kReadRows; ++k) {
+    const int64_t out_row = row0 + k;
+    rows[k] = -1;
+    if (out_row >= p.rows) continue;
+    while (slot + 1 < p.slots && out_row >= p.row_starts[slot + 1]) ++slot;
+    const int64_t place = out_row - p.row_starts[slot];
+    if (place >= 0 && out_row < p.row_starts[slot + 1])
+      rows[k] = pool_row(p.pages, p.table, p.table_stride, p.table_width, slot, p.first_rows[slot] + place);
+    if (rows[k] < 0 && lane == 0) atomicOr(p.flag, kFlagRow);
   }
+  if constexpr (GROUP == 0) {
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    const uint8_t *pool = side ? p.pages.values : p.pages.keys;
-    T *to = static_cast<T *>(side ? p.values : p.keys) + out_row * D + lane * 16;
-    float x[16];
-    if constexpr (GROUP == 0) {
-      const S *from = reinterpret_cast<const S *>(pool) + row * D + lane * 16;
-      load8(from, x);
-      load8(from + 8, x + 8);
-    } else {
-      const uint2 word = *reinterpret_cast<const uint2 *>(pool + row * (D / 2) + lane * 8);
-      const __half2 pair =
-          (side ? p.pages.value_scales : p.pages.key_scales)[row * (D / GROUP) + lane / (GROUP / 16)];
-      const float scale = __low2float(pair), offset = __high2float(pair);
+    for (int k = 0; k < kReadRows; ++k) {
+      if (rows[k] < 0) continue;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const uint32_t code = ((i < 8 ? word.x : word.y) >> (4 * (i & 7))) & 15u;
-        x[i] = fmaf(scale, static_cast<float>(code) - 8.0f, offset);
+      for (int side = 0; side < 2; ++side) {
+        const S *from = reinterpret_cast<const S *>(side ? p.pages.values : p.pages.keys) + rows[k] * D + lane * 16;
+        T *to = static_cast<T *>(side ? p.values : p.keys) + (row0 + k) * D + lane * 16;
+        float x[16];
+        load8(from, x);
+        load8(from + 8, x + 8);
+        store8(to, x);
+        store8(to + 8, x + 8);
       }
     }
-    store8(to, x);
-    store8(to + 8, x + 8);
+  } else {
+    uint2 words[kReadRows][2];
+    __half2 pairs[kReadRows][2];
+#pragma unroll
+    for (int k = 0; k < kReadRows; ++k) {
+      const int64_t row = rows[k] < 0 ? 0 : rows[k];  // row 0 exists where any row does
+      if (rows[k] < 0) continue;
+      words[k][0] = *reinterpret_cast<const uint2 *>(p.pages.keys + row * (D / 2) + lane * 8);
+      words[k][1] = *reinterpret_cast<const uint2 *>(p.pages.values + row * (D / 2) + lane * 8);
+      pairs[k][0] = p.pages.key_scales[row * (D / GROUP) + lane / (GROUP / 16)];
+      pairs[k][1] = p.pages.value_scales[row * (D / GROUP) + lane / (GROUP / 16)];
+    }
+#pragma unroll
+    for (int k = 0; k < kReadRows; ++k) {
+      if (rows[k] < 0) continue;
+#pragma unroll
+      for (int side = 0; side < 2; ++side) {
+        T *to = static_cast<T *>(side ? p.values : p.keys) + (row0 + k) * D + lane * 16;
+        const float scale = __low2float(pairs[k][side]), offset = __high2float(pairs[k][side]);
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t code = ((i < 8 ? words[k][side].x : words[k][side].y) >> (4 * (i & 7))) & 15u;
+          // 2^23 + code, less 2^23 + 8: the code without a conversion.
+          x[i] = fmaf(scale, __uint_as_float(0x4B000000u | code) - 8388616.0f, offset);
+        }
+        store8(to, x);
+        store8(to + 8, x + 8);
+      }
+    }
   }
-  if (lane == 0) p.positions[out_row] = p.pages.positions[row];
+#pragma unroll
+  for (int k = 0; k < kReadRows; ++k)
+    if (rows[k] >= 0 && lane == 0) p.positions[row0 + k] = p.pages.positions[rows[k]];
+}
+
+template <typename T, int D, int GROUP>
+void launch_append_rows(const AppendParam &p, cudaStream_t stream) {
+  constexpr int kTeams = kThreads / (D / 16);
+  const int64_t parts = 2 * p.heads + p.query_heads;
+  if (p.tokens >= kManyTokens) {
+    const int64_t grid = ceil_div(p.tokens, kTeams) * ceil_div(parts, 4);
+    append_kernel<T, D, GROUP, true><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p);
+  } else {
+    const int64_t grid = p.tokens * ceil_div(parts, kTeams);
+    append_kernel<T, D, GROUP, false><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p);
+  }
 }
 
 template <typename T, int D>
-void launch_append(const AppendParam &p, int group, unsigned grid, cudaStream_t stream) {
+void launch_append(const AppendParam &p, int group, cudaStream_t stream) {
   switch (group) {
-    case 0: append_kernel<T, D, 0><<<grid, kThreads, 0, stream>>>(p); break;
-    case 32: append_kernel<T, D, 32><<<grid, kThreads, 0, stream>>>(p); break;
-    case 64: append_kernel<T, D, 64><<<grid, kThreads, 0, stream>>>(p); break;
+    case 0: launch_append_rows<T, D, 0>(p, stream); break;
+    case 32: launch_append_rows<T, D, 32>(p, stream); break;
+    case 64: launch_append_rows<T, D, 64>(p, stream); break;
     default:
-      if constexpr (D == 128) append_kernel<T, D, 128><<<grid, kThreads, 0, stream>>>(p);
+      if constexpr (D == 128) launch_append_rows<T, D, 128>(p, stream);
   }
 }
 
@@ -335,17 +462,14 @@ extern "C" int lrk_paged_append(const lrk_pages *pages, const int32_t *table, in
   p.rotary_dim = static_cast<int>(rotary_dim);
   p.interleaved = interleaved != 0;
   p.flag = flag;
-  const int64_t rows = kThreads / (pages->dimension / 16);
-  const int64_t grid = ceil_div(tokens * (2 * heads + query_heads), rows);
-  LRK_REQUIRE(grid < (int64_t{1} << 31), "paged append: too many rows");
+  LRK_REQUIRE(tokens * (2 * heads + query_heads) < (int64_t{1} << 31), "paged append: too many rows");
   const int group = static_cast<int>(pages->group);
-  const unsigned blocks = static_cast<unsigned>(grid);
   if (dtype == LRK_F16) {
-    if (pages->dimension == 64) launch_append<__half, 64>(p, group, blocks, stream);
-    else launch_append<__half, 128>(p, group, blocks, stream);
+    if (pages->dimension == 64) launch_append<__half, 64>(p, group, stream);
+    else launch_append<__half, 128>(p, group, stream);
   } else {
-    if (pages->dimension == 64) launch_append<__nv_bfloat16, 64>(p, group, blocks, stream);
-    else launch_append<__nv_bfloat16, 128>(p, group, blocks, stream);
+    if (pages->dimension == 64) launch_append<__nv_bfloat16, 64>(p, group, stream);
+    else launch_append<__nv_bfloat16, 128>(p, group, stream);
   }
   return launch_status("paged append");
 }
@@ -367,7 +491,7 @@ extern "C" int lrk_paged_read(const lrk_pages *pages, const int32_t *table, int6
   LRK_REQUIRE(aligned(keys, 16) && aligned(values, 16), "paged read: output rows must be 16-byte aligned");
   ReadParam p{paged::device_pages(*pages), table, table_stride, table_width, first_rows, row_starts, slots, rows,
               keys, values, positions, flag};
-  const int64_t grid = ceil_div(rows, kThreads / (pages->dimension / 16));
+  const int64_t grid = ceil_div(rows, kThreads / (pages->dimension / 16) * kReadRows);
   LRK_REQUIRE(grid < (int64_t{1} << 31), "paged read: too many rows");
   const int group = static_cast<int>(pages->group);
   const unsigned blocks = static_cast<unsigned>(grid);

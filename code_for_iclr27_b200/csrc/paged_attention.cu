@@ -796,8 +796,8 @@ template <typename T, int D, int GROUP, int NT>
 int launch_rows(const AttentionParam &p, const lrk_pages &pages, cudaStream_t stream) {
   using L = Layout<T, D, GROUP, NT>;
   auto kernel = attention_kernel<T, D, GROUP, NT>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
-  if (e != cudaSuccess) return fail(LRK_ERR_CUDA, cudaGetErrorString(e));
+  static std::atomic<uint64_t> allowed{0};  // devices, a bit each, that know the kernel's shared memory
+  if (const int status = allow_shared(kernel, L::kBytes, allowed)) return status;
   CUtensorMap maps[2] = {};
   if (GROUP == 0 && pages.pages > 0) {
     const int64_t rows = pages.pages * pages.page_size;

@@ -9,6 +9,8 @@
 // joins them in a fixed order, so the result does not depend on the arrival.
 #pragma once
 
+#include <atomic>
+
 #include "paged.cuh"
 #include "tc.cuh"
 
@@ -16,6 +18,18 @@ namespace lrk {
 namespace {
 
 using namespace paged;
+
+// cudaFuncSetAttribute once per kernel and device (it costs a microsecond a call).
+template <typename K>
+int allow_shared(K kernel, int bytes, std::atomic<uint64_t> &allowed) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess && device < 64 && (allowed.load(std::memory_order_relaxed) >> device & 1)) return LRK_OK;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return fail(LRK_ERR_CUDA, cudaGetErrorString(e));
+  if (device < 64) allowed.fetch_or(uint64_t{1} << device, std::memory_order_relaxed);
+  return LRK_OK;
+}
 
 constexpr int kCounters = 4096;    // workspace: arrival counters, then partial results
 

@@ -577,8 +577,8 @@ template <typename T, int D, int GROUP>
 int launch_tc_format(const AttentionParam &p, const lrk_pages &pages, cudaStream_t stream) {
   using L = TcLayout<T, D, GROUP>;
   auto kernel = attention_tc_kernel<T, D, GROUP>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
-  if (e != cudaSuccess) return fail(LRK_ERR_CUDA, cudaGetErrorString(e));
+  static std::atomic<uint64_t> allowed{0};  // devices, a bit each, that know the kernel's shared memory
+  if (const int status = allow_shared(kernel, L::kBytes, allowed)) return status;
   CUtensorMap maps[2] = {};
   if (GROUP == 0 && pages.pages > 0) {
     const int64_t rows = pages.pages * pages.page_size;

@@ -24,6 +24,17 @@ import numpy as np
 
 from . import operators, upload
 
+_module = None
+
+
+def _operators():
+    """operators(), looked up once: a decode step's host time counts here."""
+    global _module
+    if _module is None:
+        _module = operators()
+    return _module
+
+
 #: Bytes of an attention workspace (lrk_paged_attention_workspace_bytes).
 WORKSPACE_BYTES = 64 << 20
 
@@ -91,7 +102,7 @@ def paged_append(pages: Pages, table, lengths, new_keys, new_values, new_positio
     [tokens]; token_starts int32 [sequences + 1]: token i of sequence s, of n_s, becomes row lengths - n_s + i of its
     slots.  `rotary` (rotary_table) rotates keys and `queries` [tokens, query heads, D]; the rotated queries are
     returned.  Rows without a place, and positions outside the table, are left out and set bits of `flag` (int32 [1])."""
-    return operators().paged_append(pages.keys, pages.values, pages.positions, pages.key_scales, pages.value_scales,
+    return _operators().paged_append(pages.keys, pages.values, pages.positions, pages.key_scales, pages.value_scales,
                                     table, lengths, new_keys, new_values, new_positions, token_starts, flag, rotary,
                                     interleaved, queries)
 
@@ -104,14 +115,14 @@ def paged_attention(pages: Pages, table, lengths, queries, token_starts, workspa
     to D ** -0.5; workspace: attention_workspace."""
     if scale is None:
         scale = queries.shape[2] ** -0.5
-    return operators().paged_attention(pages.keys, pages.values, pages.positions, pages.key_scales, pages.value_scales,
+    return _operators().paged_attention(pages.keys, pages.values, pages.positions, pages.key_scales, pages.value_scales,
                                        table, lengths, queries, token_starts, workspace, flag, scale, causal)
 
 
 def paged_read(pages: Pages, table, first_rows, row_starts, rows: int, dtype, flag):
     """(keys, values [rows, D] of `dtype`, positions float32 [rows]): of each slot s, row_starts[s + 1] - row_starts[s]
     rows from first_rows[s] on (both int32; `rows` is row_starts[-1]), back to back."""
-    return operators().paged_read(pages.keys, pages.values, pages.positions, pages.key_scales, pages.value_scales,
+    return _operators().paged_read(pages.keys, pages.values, pages.positions, pages.key_scales, pages.value_scales,
                                   table, first_rows, row_starts, rows, dtype, flag)
 
 
