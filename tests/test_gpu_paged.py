@@ -709,3 +709,47 @@ def test_paged_cache_through_its_life(cuda, bits):
     with pytest.raises(ValueError):
         cache.advance([1])
     assert cache.free_pages() == 400 and not cache.rows.any()
+
+
+@pytest.mark.parametrize("bits,group", [(16, 64), (4, 32), (4, 128)])
+def test_example(cuda, bits, group):
+    """The example's whole path: audit, pages, decode steps, audit.  16-bit pages against themselves differ by nothing;
+    4-bit rows, half a step of sixteen levels off each, by a tenth of the outputs' norm or so (a step is some 5 sigma /
+    15, its error a step / sqrt(12): 0.1 sigma, in keys and values both)."""
+    from code_for_iclr27_b200.paged_example import run
+
+    result = run(layers=2, rows=1024, steps=4, bits=bits, group=group)
+    assert result["rows"] == 2 * 8 * (1024 + 4) - result["evicted"]
+    assert result["rows_after_audit"] == result["rows"] - 2 * 8
+    assert result["relative_error"] == 0 if bits == 16 else 0 < result["relative_error"] < 0.3
+
+
+def test_attention_in_a_cuda_graph(cuda):
+    """A captured step (append and attention) replays on new inputs in place."""
+    import torch
+
+    from code_for_iclr27_b200.paged import attention_workspace, paged_append, paged_attention, rotary_table
+
+    case = Case(cuda, 4, "bf16", 128, 64, 64, 2, [700, 650], seed=21)
+    rotary, workspace, starts = rotary_table(1000, 128, 10000.0, cuda), attention_workspace(cuda), case.starts([1])
+    joint = torch.zeros(1, 12, 128, dtype=torch.bfloat16, device=cuda)
+    position = torch.tensor([699], device=cuda)
+
+    def step():
+        turned = paged_append(case.pages, case.table, case.lengths, joint[:, 8:10], joint[:, 10:], position, starts, case.flag,
+                              rotary, False, joint[:, :8])
+        return paged_attention(case.pages, case.table, case.lengths, turned, starts, workspace, case.flag)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in range(3):
+        joint.copy_(torch.randn(1, 12, 128, generator=torch.Generator().manual_seed(seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [t.clone() for t in held]
+        direct = step()
+        assert torch.equal(replayed[0], direct[0]) and torch.equal(replayed[1], direct[1])
+    assert int(case.flag.item()) == 0
