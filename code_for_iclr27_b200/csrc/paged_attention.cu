@@ -64,7 +64,7 @@ struct Layout {
   static constexpr int kQuery = NT * (D / 16) * 32 * 8;
   // Blocks on an SM, by registers (4-bit rows: 96, 168 and 255 a thread), and
   // one or two stages a warp, as their share of shared memory holds.
-  static constexpr int kBlocksPerSm = GROUP ? (NT == 1 ? 5 : NT == 2 ? 3 : 2) : (NT <= 2 ? 3 : 2);
+  static constexpr int kBlocksPerSm = GROUP ? (NT == 1 ? 4 : NT == 2 ? 3 : 2) : (NT <= 2 ? 3 : 2);
   static constexpr int kControl = 416;  // bytes of Control
   static constexpr int kFixed = kQuery + kGroups * kRows * 8 + kRows * 8 + 2 * kWarps * kRows * 4 + kControl;
   static constexpr int kFit = ((232448 / kBlocksPerSm - 1024) / 128 * 128 - kFixed) / kStage / kWarps;
@@ -403,7 +403,7 @@ struct Consumer {
         const uint8_t *at = values_at + gi * (GROUP / 2) + g * (GROUP / 16);
         constexpr int kWords = GROUP == 128 ? 2 : 1;
         constexpr int kBytes = GROUP / 16 / kWords;  // of a word that are used
-        uint32_t x[4][kWords];
+        uint32_t x[4][kWords], both_lo = 0, both_hi = 0;
         const uint8_t *rows[4] = {at + token * L::kRowBytes, at + other * L::kRowBytes,
                                   at + (token + 8) * L::kRowBytes, at + (other + 8) * L::kRowBytes};
 #pragma unroll
@@ -415,10 +415,18 @@ struct Consumer {
         for (int word = 0; word < kWords; ++word)
 #pragma unroll
           for (int k = 0; k < kBytes; ++k) {
-            const uint32_t select = k * 0x0011u + (4 + k) * 0x1100u;
-            const uint32_t lo = __byte_perm(x[0][word], x[1][word], select);
-            const uint32_t hi = __byte_perm(x[2][word], x[3][word], select);
-            const uint32_t a[4] = {lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u};
+            // Both rows' byte k as halves: its low nibble is the upper operand
+            // row; the whole byte, low + 16 high, is the lower one, and what is
+            // too much there is taken off the output once, at the end.
+            uint32_t lo, hi;
+            if ((k & 1) == 0) {
+              both_lo = __byte_perm(x[0][word], x[1][word], k ? 0x7632 : 0x5410);
+              both_hi = __byte_perm(x[2][word], x[3][word], k ? 0x7632 : 0x5410);
+              lo = both_lo & 0x00ff00ffu, hi = both_hi & 0x00ff00ffu;
+            } else {
+              lo = __byte_perm(both_lo, 0, 0x4341), hi = __byte_perm(both_hi, 0, 0x4341);
+            }
+            const uint32_t a[4] = {lo & 0x000f000fu, lo, hi & 0x000f000fu, hi};
             const int m = gi * (GROUP / 16) + word * kBytes + k;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -723,7 +731,7 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
             for (int k = 0; k < GROUP / 16; ++k) {
               const int m = gi * (GROUP / 16) + k;
               float2 pair = make_float2(weight * fmaf(c.out[m][nt][i], 0x1p24f, rest),
-                                        weight * fmaf(c.out[m][nt][i + 2], 0x1p20f, rest));
+                                        weight * fmaf(c.out[m][nt][i + 2] - c.out[m][nt][i], 0x1p20f, rest));
               *reinterpret_cast<float2 *>(to + gi * GROUP + g * (GROUP / 8) + 2 * k) = pair;
             }
           }
