@@ -6,7 +6,8 @@ names and signatures:
 
   _C         temporal_probabilities, temporal_risk, append, compact, pool,
              merge, pack, batch_append (+ refine, topk_smallest,
-             temporal_scores, project_values, logits, compact_layers)
+             temporal_scores, project_values, logits, compact_layers,
+             paged_append, paged_attention, paged_read)
   _legacy_C  append_flattened_cache, compact_flattened_kv, decision_risk_scores
   _host      register_host, unregister_host
 

@@ -10,7 +10,11 @@
 // values per 4-bit row at D = 128, group 64; 512 in 16 bits) for 4 D flops per
 // query head, so memory bounds it if the 4-bit codes can be unpacked as fast
 // as they arrive: at the copy rate about 40 codes per SM and clock, three
-// instructions per code.  Hence the shape of the arithmetic:
+// instructions per code.  Measured (32 requests of 33,768 rows a head, 8 query
+// heads a KV head, group 128): 247 us, 4.76 TB/s, 73 % of the copy rate, at 58 %
+// of the issue slots and 60 % of the integer pipe; copies alone, with nothing
+// computed, 203 us.  In 16 bits (8 ragged requests) 5.6 TB/s.  Hence the shape
+// of the arithmetic:
 //
 // * S^T = K Q^T and O^T = V^T P^T on m16n8k16 matrix instructions with the
 //   cache as the 16-row operand A, straight from registers, and the (few)
@@ -28,7 +32,12 @@
 //   the subtraction of 8 sum f16(p scale_g) by one more matrix instruction per
 //   group with ones as A, so that it cancels exactly what was rounded.
 //
-// Tiles are 32 rows; how they are split over the blocks: paged_attention.cuh.
+// Tiles are 32 rows; every warp moves its own (bulk copies, or TMA boxes with a
+// 128-byte swizzle for 16-bit rows) into one or two stages of its own, so the
+// warps of a block meet only at a unit's ends.  How the tiles are split over the
+// blocks: paged_attention.cuh.  Measured on the way: a feeding warp per block
+// (16 consumers and 4 feeders an SM) 296 us; twenty warps at 96 registers, with
+// spills, 276; sixteen at 128 registers 247.
 #include <cuda.h>
 
 #include <algorithm>
@@ -47,7 +56,11 @@ using namespace paged;
 constexpr int kTile = 32;   // rows per tile
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMatrixRows = 32;    // more query rows a slot than this: paged_attention_tc.cu
+// More query rows a slot than this go to paged_attention_tc.cu.  At 64 rows this
+// file's kernel takes 54, 82 and 40 us (one request of 16,384 rows a head,
+// D = 128; 24 of 4,000, D = 64; two of 8,192 in 16 bits) and that one 59, 99 and
+// 44; at 96 rows 68, 115 and 57 against 72, 107 and 51.
+constexpr int kMatrixRows = 64;
 constexpr int kMinTiles = kWarps;  // tiles per block, at least
 constexpr int kCrossing = 10;      // a second unit's cost in tiles: its start, its end, its join
 
@@ -62,8 +75,9 @@ struct Layout {
   static constexpr int kPitch = D + 4;
   static constexpr int kScratch = kWarps * 8 * kPitch * 4;
   static constexpr int kQuery = NT * (D / 16) * 32 * 8;
-  // Blocks on an SM, by registers (4-bit rows: 96, 168 and 255 a thread), and
-  // one or two stages a warp, as their share of shared memory holds.
+  // Blocks on an SM, by registers (4-bit rows: 128, 168 and 255 a thread), and
+  // one or two stages a warp, as their share of shared memory holds.  16-bit
+  // rows: three blocks 57 us, two 59 (8 ragged requests).
   static constexpr int kBlocksPerSm = GROUP ? (NT == 1 ? 4 : NT == 2 ? 3 : 2) : (NT <= 2 ? 3 : 2);
   static constexpr int kControl = 416;  // bytes of Control
   static constexpr int kFixed = kQuery + kGroups * kRows * 8 + kRows * 8 + 2 * kWarps * kRows * 4 + kControl;
@@ -822,7 +836,8 @@ int launch_rows(const AttentionParam &p, const lrk_pages &pages, cudaStream_t st
   return launch_status("paged attention");
 }
 
-// Query rows per block by the rows that a slot has on average: 8, 16 or 32.
+// Query rows per block by the rows that a slot has on average: 8, 16 or 32, the
+// columns of the matrix instructions' B; rows that there are not cost as much.
 template <typename T, int D, int GROUP>
 int launch_format(const AttentionParam &p, const lrk_pages &pages, int64_t tokens, int64_t sequences,
                   cudaStream_t stream) {
