@@ -73,18 +73,19 @@ __device__ __forceinline__ void load_floats(const float *from, float *x) {
   x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
 }
 
-// A lane's 16 channels' rotation: x' = x cosine + other sine, where `other` is
-// the pair's other channel and the sine carries the sign.
+// The rotation of a lane's two chunks of 8 channels: x' = x cosine + other sine,
+// where `other` is the pair's other channel and the sine carries the sign.
 struct Turn {
   float cosine[16], sine[16];
-  bool turns[2];  // whether the first and the last 8 channels are rotated
+  bool turns[2];  // whether each chunk is rotated
 };
 
-__device__ __forceinline__ void load_turn(const AppendParam &p, const float *table, int first, Turn &turn) {
+template <int D, int CHUNKS>
+__device__ __forceinline__ void load_turn(const AppendParam &p, const float *table, int lane, Turn &turn) {
   const int pairs = p.rotary_dim >> 1;
 #pragma unroll
-  for (int part = 0; part < 2; ++part) {
-    const int c = first + 8 * part;
+  for (int part = 0; part < CHUNKS; ++part) {
+    const int c = lane * 8 + part * (D / 2);
     float *cosine = turn.cosine + 8 * part, *sine = turn.sine + 8 * part;
     turn.turns[part] = table != nullptr && c < p.rotary_dim;
     if (!turn.turns[part]) continue;
@@ -118,64 +119,83 @@ __device__ __forceinline__ void unpack8(const uint4 &raw, float *x) {
   for (int i = 0; i < 8; ++i) x[i] = to_float<T>(e[i]);
 }
 
-// Quantises 16 channels per lane; the group / 16 lanes of a group are
-// neighbours.  Stores the lane's 8 bytes of codes and, once per group, the
-// scale and offset; a negative row stores nothing.
-template <int D, int GROUP>
-__device__ __forceinline__ void store_codes(uint8_t *codes, __half2 *scales, int64_t row, int lane, const float *x) {
-  float lo = min_nan(x[0], x[1], x[2]), hi = max_nan(x[0], x[1], x[2]);
-#pragma unroll
-  for (int i = 3; i < 15; i += 2) {
-    lo = min_nan(lo, x[i], x[i + 1]);
-    hi = max_nan(hi, x[i], x[i + 1]);
-  }
-  lo = min_nan(lo, x[15]);
-  hi = max_nan(hi, x[15]);
-#pragma unroll
-  for (int step = 1; step < GROUP / 16; step <<= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, step));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, step));
-  }
-  __half scale = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
-  const float step = __half2float(scale);
-  __half offset = __float2half_rn(__fadd_rn(lo, 8.0f * step));
-  const bool fine = !__hisinf(scale) && !__hisnan(scale) && !__hisinf(offset) && !__hisnan(offset);
-  const float inverse = step > 0.0f ? __frcp_rn(step) : 0.0f;
-  const float centre = __half2float(offset);
-  // Held to [-8, 7] and added to 1.5 * 2^23 + 8, a level leaves its code, rounded
-  // to nearest even, in the sum's last bits; a word is sum code_i 16^i.
+// Code words of 8 channels: levels held to [-8, 7] and added to 1.5 * 2^23 + 8
+// leave their codes, rounded to nearest even, in the sums' last bits; the word is
+// sum code_i 16^i.
+__device__ __forceinline__ uint32_t code_word(const float *x, float centre, float inverse) {
   constexpr float kMagic = 12582920.0f;
   constexpr uint32_t kMagicBits = 0x4B400000u;  // of 1.5 * 2^23
-  uint32_t word[2] = {0, 0};
+  uint32_t word = 0;
 #pragma unroll
-  for (int i = 7; i >= 0; --i)
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const float level = __fmul_rn(__fsub_rn(x[8 * w + i], centre), inverse);
-      word[w] = word[w] * 16 + __float_as_uint(__fadd_rn(fminf(fmaxf(level, -8.0f), 7.0f), kMagic));
-    }
-#pragma unroll
-  for (int w = 0; w < 2; ++w) word[w] -= kMagicBits * 0x11111111u;
-  if (!fine) {
-    word[0] = word[1] = 0;
-    scale = offset = __ushort_as_half(0x7fff);
+  for (int i = 7; i >= 0; --i) {
+    const float level = __fmul_rn(__fsub_rn(x[i], centre), inverse);
+    word = word * 16 + __float_as_uint(__fadd_rn(fminf(fmaxf(level, -8.0f), 7.0f), kMagic));
   }
-  if (row < 0) return;
-  *reinterpret_cast<uint2 *>(codes + row * (D / 2) + lane * 8) = make_uint2(word[0], word[1]);
-  if (lane % (GROUP / 16) == 0) scales[row * (D / GROUP) + lane / (GROUP / 16)] = __halves2half2(scale, offset);
+  return word - kMagicBits * 0x11111111u;
 }
 
-// D / 16 neighbouring lanes take a row of keys, values or queries, 16 channels
-// each, so that a group's minimum and maximum are a few shuffles; the other half
-// of a rotated pair is read once more (from L1).  BY_TOKENS: a block takes as many tokens as it has such lane groups and
+// Quantises a lane's two chunks of 8 channels (lane * 8 and D / 2 after that); a
+// group is GROUP / 8 neighbouring lanes' chunks, or the whole row.  Stores the
+// codes and, once per group, the scale and offset; a negative row stores nothing.
+template <int D, int GROUP>
+__device__ __forceinline__ void store_codes(uint8_t *codes, __half2 *scales, int64_t row, int lane, const float *x) {
+  constexpr bool kWhole = GROUP == D;
+  constexpr int kLanes = kWhole ? D / 16 : GROUP / 8;
+  float lo[2], hi[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float *y = x + 8 * k;
+    lo[k] = min_nan(min_nan(y[0], y[1], y[2]), min_nan(y[3], y[4], y[5]), min_nan(y[6], y[7]));
+    hi[k] = max_nan(max_nan(y[0], y[1], y[2]), max_nan(y[3], y[4], y[5]), max_nan(y[6], y[7]));
+  }
+  if (kWhole) {
+    lo[0] = min_nan(lo[0], lo[1]);
+    hi[0] = max_nan(hi[0], hi[1]);
+  }
+  __half scale[2], offset[2];
+  uint32_t word[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (kWhole && k == 1) {
+      scale[1] = scale[0], offset[1] = offset[0];
+    } else {
+#pragma unroll
+      for (int step = 1; step < kLanes; step <<= 1) {
+        lo[k] = min_nan(lo[k], __shfl_xor_sync(0xffffffffu, lo[k], step));
+        hi[k] = max_nan(hi[k], __shfl_xor_sync(0xffffffffu, hi[k], step));
+      }
+      scale[k] = __float2half_rn(__fmul_rn(__fsub_rn(hi[k], lo[k]), 1.0f / 15.0f));
+      offset[k] = __float2half_rn(__fadd_rn(lo[k], 8.0f * __half2float(scale[k])));
+    }
+    const float step = __half2float(scale[k]);
+    const bool fine = !__hisinf(scale[k]) && !__hisnan(scale[k]) && !__hisinf(offset[k]) && !__hisnan(offset[k]);
+    word[k] = fine ? code_word(x + 8 * k, __half2float(offset[k]), step > 0.0f ? __frcp_rn(step) : 0.0f) : 0u;
+    if (!fine && !(kWhole && k == 0)) scale[k] = offset[k] = __ushort_as_half(0x7fff);
+    if (kWhole && k == 1 && !fine) scale[0] = offset[0] = __ushort_as_half(0x7fff);
+  }
+  if (row < 0) return;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    *reinterpret_cast<uint32_t *>(codes + row * (D / 2) + lane * 4 + k * (D / 4)) = word[k];
+    if (lane % kLanes == 0 && !(kWhole && k == 1))
+      scales[row * (D / GROUP) + (lane * 8 + k * (D / 2)) / GROUP] = __halves2half2(scale[k], offset[k]);
+  }
+}
+
+// D / 16 neighbouring lanes take a row of keys, values or queries, two chunks of 8
+// channels each, D / 2 apart: every load and store is contiguous over the lanes,
+// and the pairs (j, j + D/2) of a full rotation meet in one lane (those of a
+// shorter one are read once more, from L1).  BY_TOKENS: a block takes as many tokens as it has such lane groups and
 // four rows (heads) of each, so that a token's cosines and sines are read once,
 // all four rows are in flight at a time, and a head's appended rows are written
 // side by side.  Otherwise (few tokens) a block takes one token's rows.
-template <typename T, int D, int GROUP, bool BY_TOKENS>
-__global__ __launch_bounds__(kThreads) void append_kernel(const AppendParam p) {
+// INSIDE: pairs (j, j + D/2) over all channels, which lie in one lane and share
+// their cosines; four rows then fit 96 registers, five blocks an SM.
+template <typename T, int D, int GROUP, bool BY_TOKENS, bool INSIDE>
+__global__ __launch_bounds__(kThreads, BY_TOKENS ? (INSIDE ? 5 : 4) : 1) void append_kernel(const AppendParam p) {
   constexpr int kLanes = D / 16, kTeams = kThreads / kLanes;
   constexpr int kRows = BY_TOKENS ? 4 : 1;
-  const int lane = threadIdx.x % kLanes, team = threadIdx.x / kLanes, first = lane * 16;
+  const int lane = threadIdx.x % kLanes, team = threadIdx.x / kLanes, first = lane * 8;
   const int parts = 2 * p.heads + p.query_heads;
   // Blocks of the same tokens follow one another, so that the rows read (and
   // the queries written) at a time lie together.
@@ -199,9 +219,9 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const AppendParam p) {
                                      (part - 2 * p.heads) * p.query_head;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const int c = first + 8 * k;
+      const int c = first + k * (D / 2);
       raw[r][k] = *reinterpret_cast<const uint4 *>(from + c);
-      if (!is_value && !p.interleaved && c < p.rotary_dim)
+      if (!INSIDE && !is_value && !p.interleaved && c < p.rotary_dim)
         pair[r][k] = *reinterpret_cast<const uint4 *>(from + (c < half ? c + half : c - half));
     }
   }
@@ -212,7 +232,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const AppendParam p) {
     lost = true;
   }
   Turn turn;
-  load_turn(p, turned ? p.rotary + position * p.rotary_dim : nullptr, first, turn);
+  load_turn<D, INSIDE ? 1 : 2>(p, turned ? p.rotary + position * p.rotary_dim : nullptr, lane, turn);
   if (part0 < 2 * p.heads) {
     const int64_t sequence = find_sequence(p, token);
     const int64_t start = p.token_starts[sequence], count = p.token_starts[sequence + 1] - start;
@@ -240,19 +260,29 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const AppendParam p) {
     unpack8<T>(raw[r][1], x + 8);
     if (!is_value) {
       if (lost && live && lane == 0 && part < parts) atomicOr(p.flag, kFlagPosition);
+      if constexpr (INSIDE) {
+        if (turned)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        if (!turn.turns[k]) continue;
-        float other[8], *own = x + 8 * k;
-        if (p.interleaved) {
+          for (int i = 0; i < 8; ++i) {
+            const float a = x[i], b = x[8 + i], cosine = turn.cosine[i], sine = turn.sine[i];  // the first one's: -sin
+            x[i] = __fadd_rn(__fmul_rn(a, cosine), __fmul_rn(b, sine));
+            x[8 + i] = __fsub_rn(__fmul_rn(b, cosine), __fmul_rn(a, sine));
+          }
+      } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) other[i] = own[i ^ 1];
-        } else {
-          unpack8<T>(pair[r][k], other);
+        for (int k = 0; k < 2; ++k) {
+          if (!turn.turns[k]) continue;
+          float other[8], *own = x + 8 * k;
+          if (p.interleaved) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) other[i] = own[i ^ 1];
+          } else {
+            unpack8<T>(pair[r][k], other);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            own[i] = __fadd_rn(__fmul_rn(own[i], turn.cosine[8 * k + i]), __fmul_rn(other[i], turn.sine[8 * k + i]));
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          own[i] = __fadd_rn(__fmul_rn(own[i], turn.cosine[8 * k + i]), __fmul_rn(other[i], turn.sine[8 * k + i]));
       }
     }
     if (is_key || is_value) {
@@ -262,7 +292,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const AppendParam p) {
         if (row >= 0) {
           T *to = reinterpret_cast<T *>(pool) + row * D + first;
           store8(to, x);
-          store8(to + 8, x + 8);
+          store8(to + D / 2, x + 8);
         }
       } else if constexpr (BY_TOKENS) {
         store_codes<D, GROUP>(pool, is_key ? p.pages.key_scales : p.pages.value_scales, row, lane, x);
@@ -271,7 +301,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const AppendParam p) {
     } else if (live && !lost && part < parts) {
       T *to = static_cast<T *>(p.out_queries) + (token * p.query_heads + (part - 2 * p.heads)) * D + first;
       store8(to, x);
-      store8(to + 8, x + 8);
+      store8(to + D / 2, x + 8);
     }
     if constexpr (GROUP != 0 && !BY_TOKENS) {
       // The warp's rows differ, and every lane takes part in the groups'
@@ -328,44 +358,49 @@ __global__ __launch_bounds__(kThreads) void read_kernel(const ReadParam p) {
       if (rows[k] < 0) continue;
 #pragma unroll
       for (int side = 0; side < 2; ++side) {
-        const S *from = reinterpret_cast<const S *>(side ? p.pages.values : p.pages.keys) + rows[k] * D + lane * 16;
-        T *to = static_cast<T *>(side ? p.values : p.keys) + (row0 + k) * D + lane * 16;
+        const S *from = reinterpret_cast<const S *>(side ? p.pages.values : p.pages.keys) + rows[k] * D + lane * 8;
+        T *to = static_cast<T *>(side ? p.values : p.keys) + (row0 + k) * D + lane * 8;
         float x[16];
         load8(from, x);
-        load8(from + 8, x + 8);
+        load8(from + D / 2, x + 8);
         store8(to, x);
-        store8(to + 8, x + 8);
+        store8(to + D / 2, x + 8);
       }
     }
   } else {
-    uint2 words[kReadRows][2];
-    __half2 pairs[kReadRows][2];
+    uint32_t words[kReadRows][2][2];
+    __half2 pairs[kReadRows][2][2];
 #pragma unroll
     for (int k = 0; k < kReadRows; ++k) {
-      const int64_t row = rows[k] < 0 ? 0 : rows[k];  // row 0 exists where any row does
       if (rows[k] < 0) continue;
-      words[k][0] = *reinterpret_cast<const uint2 *>(p.pages.keys + row * (D / 2) + lane * 8);
-      words[k][1] = *reinterpret_cast<const uint2 *>(p.pages.values + row * (D / 2) + lane * 8);
-      pairs[k][0] = p.pages.key_scales[row * (D / GROUP) + lane / (GROUP / 16)];
-      pairs[k][1] = p.pages.value_scales[row * (D / GROUP) + lane / (GROUP / 16)];
+#pragma unroll
+      for (int side = 0; side < 2; ++side)
+#pragma unroll
+        for (int chunk = 0; chunk < 2; ++chunk) {
+          words[k][side][chunk] = *reinterpret_cast<const uint32_t *>((side ? p.pages.values : p.pages.keys) +
+                                                                      rows[k] * (D / 2) + lane * 4 + chunk * (D / 4));
+          pairs[k][side][chunk] = (side ? p.pages.value_scales : p.pages.key_scales)[rows[k] * (D / GROUP) +
+                                                                                     (lane * 8 + chunk * (D / 2)) / GROUP];
+        }
     }
 #pragma unroll
     for (int k = 0; k < kReadRows; ++k) {
       if (rows[k] < 0) continue;
 #pragma unroll
-      for (int side = 0; side < 2; ++side) {
-        T *to = static_cast<T *>(side ? p.values : p.keys) + (row0 + k) * D + lane * 16;
-        const float scale = __low2float(pairs[k][side]), offset = __high2float(pairs[k][side]);
-        float x[16];
+      for (int side = 0; side < 2; ++side)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint32_t code = ((i < 8 ? words[k][side].x : words[k][side].y) >> (4 * (i & 7))) & 15u;
-          // 2^23 + code, less 2^23 + 8: the code without a conversion.
-          x[i] = fmaf(scale, __uint_as_float(0x4B000000u | code) - 8388616.0f, offset);
+        for (int chunk = 0; chunk < 2; ++chunk) {
+          T *to = static_cast<T *>(side ? p.values : p.keys) + (row0 + k) * D + lane * 8 + chunk * (D / 2);
+          const float scale = __low2float(pairs[k][side][chunk]), offset = __high2float(pairs[k][side][chunk]);
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            // 2^23 + code, less 2^23 + 8: the code without a conversion.
+            const uint32_t code = (words[k][side][chunk] >> (4 * i)) & 15u;
+            x[i] = fmaf(scale, __uint_as_float(0x4B000000u | code) - 8388616.0f, offset);
+          }
+          store8(to, x);
         }
-        store8(to, x);
-        store8(to + 8, x + 8);
-      }
     }
   }
 #pragma unroll
@@ -379,10 +414,16 @@ void launch_append_rows(const AppendParam &p, cudaStream_t stream) {
   const int64_t parts = 2 * p.heads + p.query_heads;
   if (p.tokens >= kManyTokens) {
     const int64_t grid = ceil_div(p.tokens, kTeams) * ceil_div(parts, 4);
-    append_kernel<T, D, GROUP, true><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p);
+    if (p.rotary_dim == D && !p.interleaved)
+      append_kernel<T, D, GROUP, true, true><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p);
+    else
+      append_kernel<T, D, GROUP, true, false><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p);
   } else {
     const int64_t grid = p.tokens * ceil_div(parts, kTeams);
-    append_kernel<T, D, GROUP, false><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p);
+    if (p.rotary_dim == D && !p.interleaved)
+      append_kernel<T, D, GROUP, false, true><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p);
+    else
+      append_kernel<T, D, GROUP, false, false><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p);
   }
 }
 

@@ -886,13 +886,13 @@ void check_rows(const torch::Tensor &rows, const torch::Tensor &pages, int64_t d
 
 // Rotated rows into the pages (lrk_paged_append).  Returns the rotated
 // queries, if any.
-std::optional<torch::Tensor> paged_append(torch::Tensor keys, torch::Tensor values, torch::Tensor positions,
-                                          std::optional<torch::Tensor> key_scales,
-                                          std::optional<torch::Tensor> value_scales, torch::Tensor table,
-                                          torch::Tensor lengths, torch::Tensor new_keys, torch::Tensor new_values,
-                                          torch::Tensor new_positions, torch::Tensor token_starts, torch::Tensor flag,
-                                          std::optional<torch::Tensor> rotary, bool interleaved,
-                                          std::optional<torch::Tensor> queries) {
+std::optional<torch::Tensor> paged_append(const torch::Tensor &keys, const torch::Tensor &values, const torch::Tensor &positions,
+                                          const std::optional<torch::Tensor> &key_scales,
+                                          const std::optional<torch::Tensor> &value_scales, const torch::Tensor &table,
+                                          const torch::Tensor &lengths, const torch::Tensor &new_keys, const torch::Tensor &new_values,
+                                          const torch::Tensor &new_positions, const torch::Tensor &token_starts, const torch::Tensor &flag,
+                                          const std::optional<torch::Tensor> &rotary, bool interleaved,
+                                          const std::optional<torch::Tensor> &queries) {
   const lrk_pages p = pages_of(keys, values, positions, key_scales, value_scales);
   check_table(table, keys);
   check_rows(new_keys, keys, p.dimension, "new rows must be float16 or bfloat16 [tokens, heads, D]");
@@ -941,9 +941,9 @@ std::optional<torch::Tensor> paged_append(torch::Tensor keys, torch::Tensor valu
 // Attention over the pages (lrk_paged_attention): (out [tokens, query heads,
 // D], lse float32 [tokens, query heads]).
 std::tuple<torch::Tensor, torch::Tensor> paged_attention(
-    torch::Tensor keys, torch::Tensor values, torch::Tensor positions, std::optional<torch::Tensor> key_scales,
-    std::optional<torch::Tensor> value_scales, torch::Tensor table, torch::Tensor lengths, torch::Tensor queries,
-    torch::Tensor token_starts, torch::Tensor workspace, torch::Tensor flag, double scale, bool causal) {
+    const torch::Tensor &keys, const torch::Tensor &values, const torch::Tensor &positions, const std::optional<torch::Tensor> &key_scales,
+    const std::optional<torch::Tensor> &value_scales, const torch::Tensor &table, const torch::Tensor &lengths, const torch::Tensor &queries,
+    const torch::Tensor &token_starts, const torch::Tensor &workspace, const torch::Tensor &flag, double scale, bool causal) {
   const lrk_pages p = pages_of(keys, values, positions, key_scales, value_scales);
   check_table(table, keys);
   check_rows(queries, keys, p.dimension, "queries must be float16 or bfloat16 [tokens, heads, D]");
@@ -974,9 +974,9 @@ std::tuple<torch::Tensor, torch::Tensor> paged_attention(
 // Rows of the pages in the packed layout (lrk_paged_read): (keys, values
 // [rows, D] of `dtype`, positions float32 [rows]).
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> paged_read(
-    torch::Tensor keys, torch::Tensor values, torch::Tensor positions, std::optional<torch::Tensor> key_scales,
-    std::optional<torch::Tensor> value_scales, torch::Tensor table, torch::Tensor first_rows, torch::Tensor row_starts,
-    int64_t rows, at::ScalarType dtype, torch::Tensor flag) {
+    const torch::Tensor &keys, const torch::Tensor &values, const torch::Tensor &positions, const std::optional<torch::Tensor> &key_scales,
+    const std::optional<torch::Tensor> &value_scales, const torch::Tensor &table, const torch::Tensor &first_rows, const torch::Tensor &row_starts,
+    int64_t rows, at::ScalarType dtype, const torch::Tensor &flag) {
   const lrk_pages p = pages_of(keys, values, positions, key_scales, value_scales);
   check_table(table, keys);
   const int64_t slots = table.size(0);
