@@ -11,8 +11,8 @@
 // query head, so memory bounds it if the 4-bit codes can be unpacked as fast
 // as they arrive: at the copy rate about 40 codes per SM and clock, three
 // instructions per code.  Measured (32 requests of 33,768 rows a head, 8 query
-// heads a KV head, group 128): 247 us, 4.76 TB/s, 73 % of the copy rate, at 58 %
-// of the issue slots and 60 % of the integer pipe; copies alone, with nothing
+// heads a KV head, group 128): 257 us, 4.57 TB/s, 70 % of the copy rate, at 60 %
+// of the issue slots and of the integer pipe; copies alone, with nothing
 // computed, 203 us.  In 16 bits (8 ragged requests) 5.6 TB/s.  Hence the shape
 // of the arithmetic:
 //
@@ -37,7 +37,7 @@
 // warps of a block meet only at a unit's ends.  How the tiles are split over the
 // blocks: paged_attention.cuh.  Measured on the way: a feeding warp per block
 // (16 consumers and 4 feeders an SM) 296 us; twenty warps at 96 registers, with
-// spills, 276; sixteen at 128 registers 247.
+// spills, 276; sixteen at 128 registers 257.
 #include <cuda.h>
 
 #include <algorithm>
@@ -417,7 +417,7 @@ struct Consumer {
         const uint8_t *at = values_at + gi * (GROUP / 2) + g * (GROUP / 16);
         constexpr int kWords = GROUP == 128 ? 2 : 1;
         constexpr int kBytes = GROUP / 16 / kWords;  // of a word that are used
-        uint32_t x[4][kWords], both_lo = 0, both_hi = 0;
+        uint32_t x[4][kWords];
         const uint8_t *rows[4] = {at + token * L::kRowBytes, at + other * L::kRowBytes,
                                   at + (token + 8) * L::kRowBytes, at + (other + 8) * L::kRowBytes};
 #pragma unroll
@@ -429,18 +429,12 @@ struct Consumer {
         for (int word = 0; word < kWords; ++word)
 #pragma unroll
           for (int k = 0; k < kBytes; ++k) {
-            // Both rows' byte k as halves: its low nibble is the upper operand
-            // row; the whole byte, low + 16 high, is the lower one, and what is
-            // too much there is taken off the output once, at the end.
-            uint32_t lo, hi;
-            if ((k & 1) == 0) {
-              both_lo = __byte_perm(x[0][word], x[1][word], k ? 0x7632 : 0x5410);
-              both_hi = __byte_perm(x[2][word], x[3][word], k ? 0x7632 : 0x5410);
-              lo = both_lo & 0x00ff00ffu, hi = both_hi & 0x00ff00ffu;
-            } else {
-              lo = __byte_perm(both_lo, 0, 0x4341), hi = __byte_perm(both_hi, 0, 0x4341);
-            }
-            const uint32_t a[4] = {lo & 0x000f000fu, lo, hi & 0x000f000fu, hi};
+            const uint32_t select = k * 0x0011u + (4 + k) * 0x1100u;
+            const uint32_t lo = __byte_perm(x[0][word], x[1][word], select);
+            const uint32_t hi = __byte_perm(x[2][word], x[3][word], select);
+            // (A whole byte, low + 16 high, as the lower operand row would save a
+            // mask, but its sixteen times larger sums lose the output's precision.)
+            const uint32_t a[4] = {lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u};
             const int m = gi * (GROUP / 16) + word * kBytes + k;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -745,7 +739,7 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
             for (int k = 0; k < GROUP / 16; ++k) {
               const int m = gi * (GROUP / 16) + k;
               float2 pair = make_float2(weight * fmaf(c.out[m][nt][i], 0x1p24f, rest),
-                                        weight * fmaf(c.out[m][nt][i + 2] - c.out[m][nt][i], 0x1p20f, rest));
+                                        weight * fmaf(c.out[m][nt][i + 2], 0x1p20f, rest));
               *reinterpret_cast<float2 *>(to + gi * GROUP + g * (GROUP / 8) + 2 * k) = pair;
             }
           }

@@ -235,6 +235,26 @@ def test_attention_many_tiles_a_block(cuda, bits, dtype, dim, group, page, group
     case.check(queries, [1] * 16, out, lse)
 
 
+@pytest.mark.parametrize("bits,dim,group", [(16, 128, 0), (4, 128, 32), (4, 128, 64), (4, 128, 128), (4, 64, 64)])
+@pytest.mark.parametrize("tokens", [1, 3, 20])
+def test_attention_long_sums_keep_precision(cuda, bits, dim, group, tokens):
+    """Nearly even weights over 33,000 rows: the output is a small rest of large sums.  In the 2-norm it may be off by
+    the output's rounding (2^-9) and the weights' (2^-9 more for bf16 weights, 2^-12 for f16)."""
+    case = Case(cuda, bits, "bf16", dim, group, 128, 1, [33000], seed=17)
+    queries = queries_of(case, [tokens], 4, spread=0.25)
+    out, _ = case.attend(queries, [tokens])
+    keys, values = case.rows[0]
+    q = queries.double().cpu().numpy()
+    want = np.empty(q.shape)
+    for i in range(tokens):
+        seen = 33000 - tokens + i + 1
+        scores = dim ** -0.5 * q[i] @ keys[:seen].T
+        weight = np.exp(scores - scores.max(-1, keepdims=True))
+        want[i] = weight @ values[:seen] / weight.sum(-1, keepdims=True)
+    off = np.linalg.norm(out.double().cpu().numpy() - want) / np.linalg.norm(want)
+    assert off <= 2.0 ** -9 + (2.0 ** -12 if bits == 4 else 2.0 ** -9), off
+
+
 @pytest.mark.parametrize("bits,dtype,dim,group", FORMATS)
 def test_attention_window_of_queries(cuda, bits, dtype, dim, group):
     """A chunk of 250 tokens at the end of a longer slot."""
