@@ -17,12 +17,12 @@
 // bf16's 8 bits would move the ends of the range by up to a third of one.
 //
 // Memory bounds both (every row read and written once), launches the small ones.
-// Measured: 19,538 tokens of 8 + 8 + 32 heads into 16-bit pages 109 us, 4.5 TB/s
-// of what has to move; 32,768 tokens into 4-bit pages and the rows back 267 us,
-// 3.4 TB/s; one layer of 276,000 4-bit rows back in bf16 38 us, 4.8 TB/s.  What
-// holds the append below the copy rate is its instructions: about 250 a warp for
-// four rows, at half the issue slots (rotations without contraction, 96 for 16
-// channels; conversions; the quantiser).
+// Measured: 19,538 tokens of 8 + 8 + 32 heads into 16-bit pages 87 us, 5.6 TB/s
+// of what has to move; 32,768 tokens into 4-bit pages and the rows back 199 us,
+// 4.5 TB/s (the quantiser costs some ten instructions a channel); one layer of
+// 276,000 4-bit rows back in bf16 34.6 us, 5.3 TB/s.  With 16 neighbouring
+// channels a lane, so that half of every rotated pair was read twice and half a
+// sector stored at a time, the three took 109, 267 and 38 us.
 #include "paged.cuh"
 
 namespace lrk {
@@ -31,9 +31,10 @@ namespace {
 using namespace paged;
 
 constexpr int kThreads = 128;
-// From here on append_kernel goes BY_TOKENS (8 KV, 32 query heads, D = 128, 16-bit
-// pages): 512 tokens 6.3 us against 5.9, 1,024 8.9 either way, 2,048 14.1 against
-// 16.5, 4,096 27.5 against 33.9.
+// From here on append_kernel goes BY_TOKENS (8 KV, 32 query heads, D = 128, into
+// 16-bit pages; into 4-bit pages and back): 512 tokens 5.6 and 11.5 us against 4.5
+// and 9.6, 1,024 6.8 and 13.5 against 6.5 and 13.4, 2,048 10.7 and 17.5 against
+// 11.7 and 21.3.
 constexpr int kManyTokens = 1024;
 
 struct AppendParam {
