@@ -201,6 +201,9 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
   }
   int64_t share;
   if (!begin<kBlockThreads, kLeastTiles, kUnitCrossing>(p, &control.sums[0][0], share, control.walk, control.segment)) return;
+  // The instructions on tensor memory want their whole warp: lanes that a wait or
+  // a branch held apart are brought together before each (__syncwarp).
+  __syncwarp();
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(
                      shared_address(&control.columns)),
@@ -268,6 +271,7 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
       if (good) atomicOr(p.flag, kFlagTimeout);
       good = false;
     }
+    __syncwarp();  // lanes leave the wait one by one
   };
 
   while (true) {
@@ -486,6 +490,7 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
       }
       sum += both.x + both.y;
       const uint32_t weights_at = lanes + L::kScoreColumn + half * (L::kHalf / 2);
+      __syncwarp();
       if constexpr (L::kHalf == 32) tc::tmem_store16(weights_at, weights);
       else tmem_store8(weights_at, weights);
       tc::tmem_wait_store();
@@ -514,13 +519,13 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
 #pragma unroll
     for (int k = 0; k < D / 2; k += 16) {
       uint32_t o[16];
+      __syncwarp();  // lanes without a query row store nothing below
       if (tiles > 0) {
         tmem_load<16>(lanes + half * (D / 2) + k, o);
       } else {
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[j] = 0;
       }
-      if (!live) continue;
       float value[16];
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -529,7 +534,9 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
         value[channel] = __uint_as_float(o[j]);
       }
       const int at = half * (D / 2) + k;
-      if (whole_unit) {
+      if (!live) {
+        // No row to write.
+      } else if (whole_unit) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) value[j] *= inverse;
         store8(static_cast<T *>(p.out) + index * D + at, value);
@@ -571,6 +578,7 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
   }
   before_sync();
   __syncthreads();
+  __syncwarp();
   if (warp == 0) {
     after_sync();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kColumns) : "memory");
