@@ -469,7 +469,8 @@ struct Consumer {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         best[nt][i] = max_nan(max_nan(s[0][nt][i], s[0][nt][i + 2], s[1][nt][i]), s[1][nt][i + 2]);
-        raises |= fmaf(best[nt][i], factor[nt][i], static_cast<float>(lift) - kMost) > top[nt][i];
+        // Also where best is NaN: top has to become NaN, since -inf stands for no rows.
+        raises |= !(fmaf(best[nt][i], factor[nt][i], static_cast<float>(lift) - kMost) <= top[nt][i]);
       }
     if (__any_sync(0xffffffffu, raises)) raise(best, largest);
 #pragma unroll

@@ -455,7 +455,8 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
       for (int k = 1; k < L::kHalf / 2; ++k) best = max_nan(best, x[k].x, x[k].y);
       // The barrier also keeps the weights from the scores that others still read.
       before_sync();
-      const bool raises = __syncthreads_or(fmaf(best, factor, -kMost) > top);
+      // (Also where best is NaN: top has to become NaN, since -inf stands for no rows.)
+      const bool raises = __syncthreads_or(!(fmaf(best, factor, -kMost) <= top));
       after_sync();
       if (raises) {
         stats[half * kBlockRows + row] = best;
