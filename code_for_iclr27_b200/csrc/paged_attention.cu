@@ -210,8 +210,7 @@ struct Consumer {
     load_words<4>(query_at + ((nt * (D / 32) + pair) * 32 + lane) * 16, b);
   }
 
-  // The largest of the value scales' bits in this lane's row of the tile.  Rows
-  // that are not visible may hold anything; they can only raise `lift` too far.
+  // The largest of the value scales' bits in this lane's row of the tile.
   __device__ __forceinline__ static uint32_t largest_scale(const uint8_t *stage, int lane) {
     uint32_t w[kNG], largest = 0;
     load_words<kNG>(stage + 2 * L::kCodes + L::kScales + lane * L::kScaleBytes, w);
@@ -461,7 +460,11 @@ struct Consumer {
             if (row + half * 16 + (i < 2 ? 0 : 8) >= seen_by[nt * 8 + 2 * (lane & 3) + (i & 1)]) s[half][nt][i] = -INFINITY;
     }
     uint32_t largest = 0;
-    if constexpr (GROUP != 0) largest = largest_scale(stage, lane);
+    if constexpr (GROUP != 0) {
+      // What lies beyond every query's rows (or, past a page of 16, was never
+      // copied) may be anything, and must not raise `lift`.
+      if (!MASKED || first_row + lane < seen_max) largest = largest_scale(stage, lane);
+    }
     bool raises = largest > plain_scale();
     float best[NT][2];
 #pragma unroll

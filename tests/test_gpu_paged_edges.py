@@ -9,7 +9,7 @@ import math
 import numpy as np
 import pytest
 
-from test_gpu_paged import FORMATS, Case, queries_of
+from test_gpu_paged import FORMATS, UNIT, Case, queries_of
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +78,81 @@ def test_lse_of_queries_that_are_not_numbers(cuda, bits, dtype, dim, group, grou
     bad[0, 1] = bad[1, 0] = True
     assert torch.isnan(out[bad]).all() and torch.isnan(lse[bad]).all()
     assert torch.isfinite(out[~bad]).all() and torch.isfinite(lse[~bad]).all()
+
+
+def compare(case, queries, counts, out, lse, scale=None, absent=None, flag=0):
+    """Case.check's bound, with what weights below f16's normal range lose (2^-22 of the largest) taken of the slot's
+    largest value in the channel instead of 1; a weight times a scale below f16's normal range loses 2^-25 (its codes
+    eight times that) beside a largest weight of 2^8.  absent: slot -> rows that are left out."""
+    dim, heads = case.dim, case.heads
+    groups = queries.shape[1] // heads
+    scale = dim ** -0.5 if scale is None else scale
+    q = queries.double().cpu().numpy()
+    got, got_lse = out.double().cpu().numpy(), lse.double().cpu().numpy()
+    name = "bf16" if str(out.dtype).endswith("bfloat16") else "f16"
+    unit = UNIT["f16"] if case.bits == 4 else UNIT[name]
+    lengths = case.lengths.cpu().tolist()
+    t = 0
+    for s, n in enumerate(counts):
+        for i in range(n):
+            for h in range(heads):
+                slot = s * heads + h
+                keep = np.arange(max(0, lengths[slot] - n + i + 1))
+                if absent and slot in absent:
+                    keep = np.setdiff1d(keep, absent[slot])
+                at = slice(h * groups, (h + 1) * groups)
+                if keep.size == 0:
+                    assert (got[t, at] == 0).all() and np.isneginf(got_lse[t, at]).all(), (s, i, h)
+                    continue
+                keys, values, sizes = case.rows[slot][0][keep], case.rows[slot][1][keep], case.sizes[slot][keep]
+                scores = scale * q[t, at] @ keys.T
+                top = scores.max(-1, keepdims=True)
+                weight = np.exp(scores - top)
+                total = weight.sum(-1, keepdims=True)
+                want, want_lse = weight @ values / total, (top + np.log(total))[:, 0]
+                d = (dim + 16) * 2.0 ** -23 * abs(scale) * (np.abs(q[t, at]) @ np.abs(keys).T).max()
+                bound = ((2 * unit + 4 * d + 2.0 ** -16) * (weight @ sizes / total) + UNIT[name] * np.abs(want) +
+                         keep.size / total * (2.0 ** -22 * case.sizes[slot].max(0) + (2.0 ** -30 if case.bits == 4 else 0)) +
+                         (2.0 ** -25 if name == "f16" else 0))
+                off = np.abs(got[t, at] - want)
+                assert (off <= bound).all(), (s, i, h, off.max(), bound.min())
+                assert (np.abs(got_lse[t, at] - want_lse) <= 2 * d + 2.0 ** -20 * (1 + np.abs(want_lse))).all(), (s, i, h)
+            t += 1
+    assert int(case.flag.item()) == flag
+
+
+def fill_unused(case, scale, offset):
+    """(scale, offset) in every row of the pages that no slot holds."""
+    import torch
+
+    used = np.zeros(tuple(case.pages.positions.shape), dtype=bool)
+    for slot, n in enumerate(case.lengths.tolist()):
+        row = np.arange(n)
+        used[case.host_table[slot, row // case.page], row % case.page] = True
+    unused = torch.from_numpy(~used).to(case.device)
+    pair = torch.tensor([scale, offset], dtype=torch.float16, device=case.device)
+    for scales in (case.pages.key_scales, case.pages.value_scales):
+        scales[unused] = pair
+
+
+@pytest.mark.parametrize("dim,group", [(128, 32), (128, 64), (128, 128), (64, 32), (64, 64)])
+@pytest.mark.parametrize("page", [16, 32, 128])
+@pytest.mark.parametrize("tokens,groups", [(1, 4), (3, 4), (7, 4), (1, 70)])
+def test_scales_beyond_a_slot_are_not_used(cuda, dim, group, page, tokens, groups):
+    """The same bits whatever the unused rows' scales hold, in pages (and, where a page of 16 rows ends a tile, in what
+    an earlier call left in shared memory), for values so small that their weights' precision would show it."""
+    import torch
+
+    lengths = [37, 7, 16, 100]
+    case = Case(cuda, 4, "bf16", dim, group, page, 1, lengths, seed=3, value_spread=lambda n: np.full(n, 1e-3))
+    large = Case(cuda, 4, "bf16", dim, group, page, 1, [1024] * 32, seed=4, value_spread=lambda n: np.full(n, 60000.0))
+    counts = [tokens] * 4
+    queries = queries_of(case, counts, groups)
+    fill_unused(case, 0.0, 0.0)
+    want, want_lse = case.attend(queries, counts)
+    compare(case, queries, counts, want, want_lse)
+    for scale, offset in ((float("nan"), float("nan")), (65504.0, 0.0), (-65504.0, 1.0), (float("inf"), float("-inf")), (0.0, 0.0)):
+        fill_unused(case, scale, offset)
+        large.attend(queries_of(large, [1] * 32, groups), [1] * 32)
+        out, lse = case.attend(queries, counts)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse), scale
