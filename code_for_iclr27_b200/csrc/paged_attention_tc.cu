@@ -10,8 +10,11 @@
 // * keys as the whole numbers n - 8, exact in f16; one accumulator per group,
 //   and scale_g S_g + offset_g sum(q)_g in float32 by the thread that holds the
 //   row's scores, so scores are as exact as with unpacked float32 rows;
-// * values as f16((offset + scale (n - 8)) / 2): halved, so that every value
-//   that f16 scales and offsets can name stays finite; the output is doubled.
+// * values as f16(2^-power (offset + scale (n - 8))), 11 bits like the weights'.
+//   The power is the block's: it brings the largest value of a segment's first
+//   tile below 2^11, and is raised (the output so far rescaled) where a later
+//   tile passes 2^15.  f16 scales and offsets name values from 2^-24 to some
+//   500,000; a fixed power would overflow or round off the ends of that.
 // Within each 8 channels both operands take the order 0 4 1 5 2 6 3 7 in which
 // a word's nibbles unpack in pairs; Q takes it too, and the output undoes it.
 // The weights go back to tensor memory as the A operand; values are the B
@@ -74,6 +77,7 @@ struct TcControl {
   uint64_t landed[3], scored, added;
   int64_t sums[2][kBlockThreads / 32];
   Walk<kBlockRows, TILE> walk;
+  int32_t tops[kBlockThreads / 32];
   uint32_t columns;
   int32_t abort;
   int32_t arrived[2];
@@ -266,6 +270,70 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
     }
     __syncwarp();
   };
+  // Unpacking: a thread keeps its chunk of 8 channels, and takes every (threads /
+  // chunks)th row.  Value rows from `seen_max` on may hold anything, and 0 NaN is
+  // NaN: they become zeros and count for nothing.
+  constexpr int kChunks = D / 8, kStep = kBlockThreads / kChunks;
+  const auto value_scales = [&](const uint8_t *stage, int r) {
+    return reinterpret_cast<const uint32_t *>(stage + 2 * L::kCodes + L::kScales)[r * L::kGroups +
+                                                                                  threadIdx.x % kChunks * 8 / GROUP];
+  };
+  // Stores the rows' values times 2^-power; whether one may pass 2^15.
+  const auto unpack_values = [&](const uint8_t *stage, int32_t first_row, int32_t seen_max, int32_t power) {
+    const int c = threadIdx.x % kChunks;
+    const __half2 down = __half2half2(__ushort_as_half(static_cast<unsigned short>((15 - power) << 10)));
+    uint32_t largest = 0;  // of the scales' bits (low half) and of the offsets', signs left out
+#pragma unroll
+    for (int r = threadIdx.x / kChunks; r < L::kTile; r += kStep) {
+      __align__(16) __half2 n[4];
+      unpack8(*reinterpret_cast<const uint32_t *>(stage + L::kCodes + L::kScales + r * (D / 2) + c * 4), n);
+      const uint32_t bits = first_row + r < seen_max ? value_scales(stage, r) : 0u;
+      largest = __vmaxu2(largest, bits & 0x7fff7fffu);
+      const __half2 pair = __hmul2(*reinterpret_cast<const __half2 *>(&bits), down);
+      const __half2 scale = __low2half2(pair), offset = __high2half2(pair);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) n[k] = __hfma2(n[k], scale, offset);
+      *reinterpret_cast<uint4 *>(shared + L::kOperandAt + L::kOperand + chunk_at(r, c, L::kTile)) =
+          *reinterpret_cast<uint4 *>(n);
+    }
+    // |v| < 2^(e - 13), e the larger of the offset's exponent field and the scale's plus 3.
+    return (largest & 0xffffu) >= static_cast<uint32_t>(26 + power) << 10 ||
+           (largest >> 16) >= static_cast<uint32_t>(29 + power) << 10;
+  };
+  // The larger exponent field of this thread's visible rows: scales' plus 3, offsets'.
+  // Those that are not finite reach their own rows, whatever the power.
+  const auto largest_scales = [&](const uint8_t *stage, int32_t first_row, int32_t seen_max) {
+    int32_t largest = 0;
+#pragma unroll 1
+    for (int r = threadIdx.x / kChunks; r < min(L::kTile, seen_max - first_row); r += kStep) {
+      const uint32_t bits = value_scales(stage, r);
+      const int32_t scale = bits >> 10 & 31, offset = bits >> 26 & 31;
+      largest = max(largest, max(scale < 31 ? scale + 3 : 0, offset < 31 ? offset : 0));
+    }
+    return largest;
+  };
+  // The power that brings the block's values below 2^11, as far as f16 can hold
+  // 2^-power.  A barrier for all.
+  const auto common_power = [&](int32_t largest) {
+    largest = __reduce_max_sync(0xffffffffu, largest);
+    if (lane == 0) control.tops[warp] = largest;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kBlockThreads / 32; ++w) largest = max(largest, control.tops[w]);
+    return max(largest - 24, -15);
+  };
+  // Multiplies the output so far.
+  const auto rescale = [&](float by) {
+#pragma unroll
+    for (int k = 0; k < D / 2; k += 16) {
+      uint32_t o[16];
+      tmem_load<16>(lanes + half * (D / 2) + k, o);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
+      tc::tmem_store16(lanes + half * (D / 2) + k, o);
+    }
+    tc::tmem_wait_store();
+  };
   const auto waits = [&](uint32_t barrier, uint32_t parity) {
     if (!wait(barrier, parity, abort)) {
       if (good) atomicOr(p.flag, kFlagTimeout);
@@ -348,18 +416,17 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
       }
     }
     float top = -INFINITY, sum = 0.0f;
+    int32_t power = 0;  // 4-bit values are held as v 2^-power
 
     for (int32_t i = 0; i < tiles; ++i, ++count) {
       const uint32_t slot = count % L::kStages;
       const int32_t first_row = (s.tile0 + i) * L::kTile;
       uint8_t *const stage = shared + L::kStageAt + slot * L::kStage;
+      bool large = false;
       const uint32_t keys_at = base + (GROUP ? L::kOperandAt : L::kStageAt + slot * L::kStage);
       const uint32_t values_at = keys_at + L::kOperand;
       waits(shared_address(&control.landed[slot]), (count / L::kStages) & 1);
       if constexpr (GROUP != 0) {
-        // Unpack: a thread keeps its chunk of channels, and takes every
-        // (threads / chunks)th row.
-        constexpr int kChunks = D / 8, kStep = kBlockThreads / kChunks;
         const int c = threadIdx.x % kChunks;
         uint8_t *const operands = shared + L::kOperandAt;
 #pragma unroll
@@ -375,21 +442,8 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
           reinterpret_cast<float4 *>(shared + L::kTableAt)[k] = make_float4(a.x, b.x, a.y, b.y);
         }
         if (i > 0) waits(added, (count - 1) & 1);  // the last tile's values have been used
-        const uint8_t *value_stage = stage + L::kCodes + L::kScales;
-        const __half2 two_halves = __float2half2_rn(0.5f);
-#pragma unroll
-        for (int r = threadIdx.x / kChunks; r < L::kTile; r += kStep) {
-          __align__(16) __half2 n[4];
-          unpack8(*reinterpret_cast<const uint32_t *>(value_stage + r * (D / 2) + c * 4), n);
-          const __half2 pair = __hmul2(
-              reinterpret_cast<const __half2 *>(value_stage + L::kCodes)[r * L::kGroups + c * 8 / GROUP], two_halves);
-          const __half2 scale = __low2half2(pair), offset = __high2half2(pair);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) n[k] = __hfma2(n[k], scale, offset);
-          // Rows beyond every query's may hold anything, and 0 NaN is NaN.
-          if (first_row + r >= s.seen_max) n[0] = n[1] = n[2] = n[3] = __float2half2_rn(0.0f);
-          *reinterpret_cast<uint4 *>(operands + L::kOperand + chunk_at(r, c, L::kTile)) = *reinterpret_cast<uint4 *>(n);
-        }
+        if (i == 0) power = common_power(largest_scales(stage, first_row, s.seen_max));
+        large = unpack_values(stage, first_row, s.seen_max, power);
       } else {
         if (i > 0) waits(added, (count - 1) & 1);
         if (warp == 1 && i + 1 < tiles) feed(s, s.tile0 + i + 1, count + 1);  // into the stage that is free now
@@ -401,7 +455,21 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       before_sync();
-      __syncthreads();
+      if constexpr (GROUP == 0) {
+        __syncthreads();
+      } else if (__syncthreads_or(large)) {
+        // Values that pass 2^15 (or scales that are not finite): a new power.
+        const int32_t next = max(power, common_power(largest_scales(stage, first_row, s.seen_max)));
+        if (next != power) {
+          after_sync();
+          if (i > 0) rescale(__int_as_float((127 + power - next) << 23));
+          power = next;
+          unpack_values(stage, first_row, s.seen_max, power);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          before_sync();
+          __syncthreads();
+        }
+      }
       after_sync();
       if (threadIdx.x == 0) {
 #pragma unroll
@@ -466,17 +534,7 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
         const float keep = top == -INFINITY ? 0.0f : exp2_fast(top - next);
         top = next;
         sum *= keep;
-        if (i > 0 && __any_sync(0xffffffffu, keep != 1.0f)) {
-#pragma unroll
-          for (int k = 0; k < D / 2; k += 16) {
-            uint32_t o[16];
-            tmem_load<16>(lanes + half * (D / 2) + k, o);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-            tc::tmem_store16(lanes + half * (D / 2) + k, o);
-          }
-          tc::tmem_wait_store();
-        }
+        if (i > 0 && __any_sync(0xffffffffu, keep != 1.0f)) rescale(keep);
         __syncthreads();  // before the maxima are written over
       }
       const float shift = top == -INFINITY ? 0.0f : -top;
@@ -515,7 +573,8 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
     const float weight_sum = stats[2 * kBlockRows + row] + stats[3 * kBlockRows + row];
     const bool whole_unit = s.starts && s.ends;
     float *partial = p.partials + (static_cast<int64_t>(blockIdx.x) * 2 + (s.starts ? 1 : 0)) * kBlockRows * (D + 2);
-    const float inverse = (weight_sum == 0.0f ? 0.0f : 1.0f / weight_sum) * (GROUP ? 2.0f : 1.0f);
+    const float restore = GROUP ? __int_as_float((127 + power) << 23) : 1.0f;
+    const float inverse = (weight_sum == 0.0f ? 0.0f : 1.0f / weight_sum) * restore;
     const int64_t index = out_row(p, s, live ? query_row : s.row0);
 #pragma unroll
     for (int k = 0; k < D / 2; k += 16) {
@@ -546,8 +605,7 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
 #pragma unroll
         for (int j = 0; j < 16; j += 4)
           *reinterpret_cast<float4 *>(partial + row * D + at + j) =
-              make_float4(value[j] * (GROUP ? 2.0f : 1.0f), value[j + 1] * (GROUP ? 2.0f : 1.0f),
-                          value[j + 2] * (GROUP ? 2.0f : 1.0f), value[j + 3] * (GROUP ? 2.0f : 1.0f));
+              make_float4(value[j] * restore, value[j + 1] * restore, value[j + 2] * restore, value[j + 3] * restore);
       }
     }
     if (live && half == 0) {

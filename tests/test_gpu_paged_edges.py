@@ -156,3 +156,55 @@ def test_scales_beyond_a_slot_are_not_used(cuda, dim, group, page, tokens, group
         large.attend(queries_of(large, [1] * 32, groups), [1] * 32)
         out, lse = case.attend(queries, counts)
         assert torch.equal(out, want) and torch.equal(lse, want_lse), scale
+
+
+def refill(case, make):
+    """New rows in every slot, appended (so quantised) as a user's are: make(n) gives float32 keys and values [n, D]."""
+    import torch
+
+    from code_for_iclr27_b200.paged import paged_append, paged_read
+
+    zero = torch.zeros(1, dtype=torch.int32, device=case.device)
+    for slot, n in enumerate(case.lengths.tolist()):
+        if n == 0:
+            continue
+        new = [torch.from_numpy(x.astype(np.float32)).to(case.dtype).to(case.device)[:, None] for x in make(n)]
+        at = slice(slot, slot + 1)
+        paged_append(case.pages, case.table[at], case.lengths[at], *new, torch.zeros(n, dtype=torch.int64, device=case.device),
+                     case.starts([n]), case.flag)
+        keys, values, _ = paged_read(case.pages, case.table[at], zero, case.starts([n]), n, torch.float32, case.flag)
+        case.rows[slot] = (keys.double().cpu().numpy(), values.double().cpu().numpy())
+        if case.bits == 16:
+            case.sizes[slot] = np.abs(case.rows[slot][1])
+        else:
+            row = np.arange(n)
+            held = case.pages.value_scales.double().cpu().numpy()[case.host_table[slot, row // case.page], row % case.page]
+            case.sizes[slot] = np.repeat(8 * held[..., 0] + np.abs(held[..., 1]), case.group, -1)
+    assert int(case.flag.item()) == 0
+
+
+FOUR_BITS = [(4, "bf16", 128, 32), (4, "bf16", 128, 64), (4, "bf16", 128, 128), (4, "bf16", 64, 32), (4, "bf16", 64, 64)]
+
+
+@pytest.mark.parametrize("bits,dtype,dim,group", FOUR_BITS)
+@pytest.mark.parametrize("groups", [4, 14, 30, 70])
+@pytest.mark.parametrize("kind", ["huge", "tiny", "rising", "falling", "mixed"])
+def test_values_of_any_magnitude(cuda, bits, dtype, dim, group, groups, kind):
+    """Values up to what a group's float16 scale and offset can name (some 500,000, far beyond float16), down to
+    1e-6, and both in one slot.  The ends of every group's range are set so that its offset stays in float16's range."""
+    rng = np.random.default_rng(5)
+    size = {"huge": lambda n: np.full(n, 5e5), "tiny": lambda n: np.full(n, 1e-6),
+            "rising": lambda n: np.geomspace(1e-6, 5e5, n), "falling": lambda n: np.geomspace(5e5, 1e-6, n),
+            "mixed": lambda n: np.where(np.arange(n) % 97 == 50, 3e5, 1e-3)}[kind]
+
+    def make(n):
+        values = rng.uniform(-0.9, 0.9, (n, dim))
+        values[:, 0::group], values[:, 1::group] = -1.0, 0.96
+        return rng.standard_normal((n, dim)), values * size(n)[:, None]
+
+    case = Case(cuda, bits, dtype, dim, group, 32, 1, [700, 40], seed=13)
+    refill(case, make)
+    queries = queries_of(case, [1, 1], groups)
+    out, lse = case.attend(queries, [1, 1])
+    assert np.isfinite(out.float().cpu().numpy()).all()
+    compare(case, queries, [1, 1], out, lse)
