@@ -31,7 +31,7 @@ int allow_shared(K kernel, int bytes, std::atomic<uint64_t> &allowed) {
   return LRK_OK;
 }
 
-constexpr int kCounters = 4096;    // workspace: arrival counters, then partial results
+constexpr int kCounters = 4096;  // workspace: arrival counters (zero between calls), then partial results
 
 // Division by a number that the host knows: n / d for n below 2^31 as a
 // product (Granlund and Montgomery's round-up method).

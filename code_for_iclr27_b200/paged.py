@@ -35,8 +35,10 @@ def _operators():
     return _module
 
 
-#: Bytes of an attention workspace (lrk_paged_attention_workspace_bytes).
+#: Bytes of an attention workspace (lrk_paged_attention_workspace_bytes), and how many of them, from the first, must be
+#: zero before its first call (every call leaves them so).
 WORKSPACE_BYTES = 64 << 20
+WORKSPACE_COUNTER_BYTES = 16 << 10
 
 
 @dataclass
@@ -88,8 +90,9 @@ def rotary_table(positions: int, rotary_dim: int, theta: float, device):
 
 
 def attention_workspace(device):
-    """A workspace for paged_attention: zeroed once, kept between calls.  Calls that may overlap (on two streams, say)
-    need one each."""
+    """A workspace for paged_attention: zeroed once, kept between calls.  Calls that may overlap (on two streams, or in
+    two graphs that are replayed at a time) need one each.  Make it outside of a graph's capture: inside, the zeroing
+    belongs to the graph."""
     import torch
 
     return torch.zeros(WORKSPACE_BYTES, dtype=torch.uint8, device=device)
@@ -222,14 +225,20 @@ class PagedCache:
         return paged_append(self.pages, self.tables[layer], self.lengths[layer], new_keys, new_values, positions,
                             self.token_starts, self.flag, rotary, interleaved, queries)
 
-    def attend(self, layer: int, queries, scale: Optional[float] = None, causal: bool = True):
-        """(out, lse) of the step's queries over one layer (paged_attention)."""
+    def attend(self, layer: int, queries, scale: Optional[float] = None, causal: bool = True, workspace=None):
+        """(out, lse) of the step's queries over one layer (paged_attention).  Without a `workspace` the cache takes one
+        that it keeps for the current stream; in a graph's capture, where neither that stream nor what a call left
+        behind says what the replays will find, memory of the graph whose counters the graph zeroes each time."""
         import torch
 
-        stream = torch.cuda.current_stream(self.device).cuda_stream
-        workspace = self._workspaces.get(stream)
-        if workspace is None:
-            workspace = self._workspaces[stream] = attention_workspace(self.device)
+        if workspace is None and torch.cuda.is_current_stream_capturing():
+            workspace = torch.empty(WORKSPACE_BYTES, dtype=torch.uint8, device=self.device)
+            workspace[:WORKSPACE_COUNTER_BYTES].zero_()
+        elif workspace is None:
+            stream = torch.cuda.current_stream(self.device).cuda_stream
+            workspace = self._workspaces.get(stream)
+            if workspace is None:
+                workspace = self._workspaces[stream] = attention_workspace(self.device)
         return paged_attention(self.pages, self.tables[layer], self.lengths[layer], queries, self.token_starts,
                                workspace, self.flag, scale, causal)
 

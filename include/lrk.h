@@ -570,8 +570,8 @@ int lrk_paged_append(const lrk_pages *pages, const int32_t *table, int64_t table
  * 16-bit pages and queries share one type.  Sums and softmax statistics are float32;
  * weights are rounded once to f16 (4-bit and f16 rows) or bf16.
  * workspace: lrk_paged_attention_workspace_bytes() bytes, 16-byte aligned,
- * zeroed once by the caller and left zeroed where it must be; calls that may
- * overlap need one each. */
+ * its first 16 KB (arrival counters) zeroed once by the caller and left zeroed
+ * by every call; calls that may overlap need one each. */
 size_t lrk_paged_attention_workspace_bytes(void);
 int lrk_paged_attention(const lrk_pages *pages, const int32_t *table, int64_t table_stride, int64_t table_width,
                         const int32_t *lengths, int64_t sequences, int64_t heads, const int32_t *token_starts,

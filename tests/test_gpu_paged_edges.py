@@ -208,3 +208,67 @@ def test_values_of_any_magnitude(cuda, bits, dtype, dim, group, groups, kind):
     out, lse = case.attend(queries, [1, 1])
     assert np.isfinite(out.float().cpu().numpy()).all()
     compare(case, queries, [1, 1], out, lse)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_captured_steps_of_a_cache(cuda, bits):
+    """Two graphs of a PagedCache's step, captured one after the other: the second may be replayed first, on streams of
+    their own, beside the cache's own calls, and each gives the bits of a direct call."""
+    import torch
+
+    from code_for_iclr27_b200.paged import PagedCache, attention_workspace
+    from test_gpu_arena import make_packed
+
+    cache = PagedCache(3, 1, 4, 128, 200, cuda, bits=bits, page_size=64, max_rows=2048)
+    cache.load(0, make_packed(cuda, seed=1))
+    cache.advance([1])
+    for layer in range(3):
+        cache.append(layer, *(queries_of_shape((1, 4, 128), seed, cuda) for seed in (3, 4)), torch.tensor([900], device=cuda))
+    queries = [queries_of_shape((1, 8, 128), seed, cuda) for seed in (1, 2)]
+    kept = attention_workspace(cuda)
+
+    def step(query, **more):
+        return [cache.attend(layer, query, **more) for layer in range(3)]
+
+    want = [step(q) for q in queries]
+    torch.cuda.synchronize()
+    graphs, held = [], []
+    junk = torch.full((256 << 20,), 0x5a, dtype=torch.uint8, device=cuda)
+    del junk
+    torch.cuda.empty_cache()  # memory that a graph's pool is given from here on may hold anything
+    for query in queries:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            held.append(step(query))
+    for workspace in getattr(cache, "_workspaces", {}).values():
+        assert int(workspace[:4 * 4096].count_nonzero()) == 0  # a direct call finds its counters at zero
+    for order in ((1, 0), (0, 1), (1, 1)):
+        for tensors in held:
+            for out, lse in tensors:
+                out.fill_(float("nan"))
+                lse.fill_(float("nan"))
+        for number in order:
+            graphs[number].replay()
+        torch.cuda.synchronize()
+        for number in order:
+            for (out, lse), (want_out, want_lse) in zip(held[number], want[number]):
+                assert torch.equal(out, want_out) and torch.equal(lse, want_lse)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        step(queries[0])
+    torch.cuda.synchronize()
+    for number in range(2):
+        for (out, lse), (want_out, want_lse) in zip(held[number], want[number]):
+            assert torch.equal(out, want_out) and torch.equal(lse, want_lse)
+    for out, want_out in zip(step(queries[1], workspace=kept), want[1]):
+        assert torch.equal(out[0], want_out[0]) and torch.equal(out[1], want_out[1])
+    cache.check_flags()
+
+
+def queries_of_shape(shape, seed, device):
+    import torch
+
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16).to(device)
