@@ -77,7 +77,6 @@ struct TcControl {
   uint64_t landed[3], scored, added;
   int64_t sums[2][kBlockThreads / 32];
   Walk<kBlockRows, TILE> walk;
-  int32_t tops[kBlockThreads / 32];
   uint32_t columns;
   int32_t abort;
   int32_t arrived[2];
@@ -270,69 +269,65 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
     }
     __syncwarp();
   };
-  // Unpacking: a thread keeps its chunk of 8 channels, and takes every (threads /
-  // chunks)th row.  Value rows from `seen_max` on may hold anything, and 0 NaN is
-  // NaN: they become zeros and count for nothing.
+  // Unpacking values: a thread keeps its chunk of 8 channels, and takes every
+  // (threads / chunks)th row.  Rows from `seen_max` on may hold anything, and
+  // 0 NaN is NaN.
   constexpr int kChunks = D / 8, kStep = kBlockThreads / kChunks;
-  const auto value_scales = [&](const uint8_t *stage, int r) {
-    return reinterpret_cast<const uint32_t *>(stage + 2 * L::kCodes + L::kScales)[r * L::kGroups +
-                                                                                  threadIdx.x % kChunks * 8 / GROUP];
-  };
-  // Stores the rows' values times 2^-power; whether one may pass 2^15.
   const auto unpack_values = [&](const uint8_t *stage, int32_t first_row, int32_t seen_max, int32_t power) {
     const int c = threadIdx.x % kChunks;
+    const uint8_t *value_stage = stage + L::kCodes + L::kScales;
     const __half2 down = __half2half2(__ushort_as_half(static_cast<unsigned short>((15 - power) << 10)));
-    uint32_t largest = 0;  // of the scales' bits (low half) and of the offsets', signs left out
 #pragma unroll
     for (int r = threadIdx.x / kChunks; r < L::kTile; r += kStep) {
       __align__(16) __half2 n[4];
-      unpack8(*reinterpret_cast<const uint32_t *>(stage + L::kCodes + L::kScales + r * (D / 2) + c * 4), n);
-      const uint32_t bits = first_row + r < seen_max ? value_scales(stage, r) : 0u;
-      largest = __vmaxu2(largest, bits & 0x7fff7fffu);
-      const __half2 pair = __hmul2(*reinterpret_cast<const __half2 *>(&bits), down);
+      unpack8(*reinterpret_cast<const uint32_t *>(value_stage + r * (D / 2) + c * 4), n);
+      const __half2 pair =
+          __hmul2(reinterpret_cast<const __half2 *>(value_stage + L::kCodes)[r * L::kGroups + c * 8 / GROUP], down);
       const __half2 scale = __low2half2(pair), offset = __high2half2(pair);
 #pragma unroll
       for (int k = 0; k < 4; ++k) n[k] = __hfma2(n[k], scale, offset);
+      if (first_row + r >= seen_max) n[0] = n[1] = n[2] = n[3] = __float2half2_rn(0.0f);
       *reinterpret_cast<uint4 *>(shared + L::kOperandAt + L::kOperand + chunk_at(r, c, L::kTile)) =
           *reinterpret_cast<uint4 *>(n);
     }
-    // |v| < 2^(e - 13), e the larger of the offset's exponent field and the scale's plus 3.
-    return (largest & 0xffffu) >= static_cast<uint32_t>(26 + power) << 10 ||
-           (largest >> 16) >= static_cast<uint32_t>(29 + power) << 10;
   };
-  // The larger exponent field of this thread's visible rows: scales' plus 3, offsets'.
-  // Those that are not finite reach their own rows, whatever the power.
-  const auto largest_scales = [&](const uint8_t *stage, int32_t first_row, int32_t seen_max) {
-    int32_t largest = 0;
-#pragma unroll 1
-    for (int r = threadIdx.x / kChunks; r < min(L::kTile, seen_max - first_row); r += kStep) {
-      const uint32_t bits = value_scales(stage, r);
-      const int32_t scale = bits >> 10 & 31, offset = bits >> 26 & 31;
-      largest = max(largest, max(scale < 31 ? scale + 3 : 0, offset < 31 ? offset : 0));
+  // The power for a tile's values, found by every warp for itself: a lane holds a
+  // 32nd of the tile's (scale, offset) pairs, signs left out.  A value is below
+  // 2^(e - 13), e the larger of the offset's exponent field and the scale's plus 3;
+  // the power stays while that is at most 2^(15 + power), and brings it below
+  // 2^(11 + power) otherwise (as far as f16 holds 2^-power).  Pairs that are not
+  // finite reach their own rows, whatever the power.
+  const auto tile_power = [&](const uint8_t *stage, int32_t first_row, int32_t seen_max, int32_t power, bool first) {
+    constexpr int kWords = L::kTile * L::kGroups / 32;
+    uint32_t w[kWords];
+    const uint8_t *from = stage + 2 * L::kCodes + L::kScales + lane * kWords * 4;
+    if constexpr (kWords == 4) {
+      const uint4 x = *reinterpret_cast<const uint4 *>(from);
+      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else {
+      const uint2 x = *reinterpret_cast<const uint2 *>(from);
+      w[0] = x.x, w[1] = x.y;
     }
-    return largest;
-  };
-  // The power that brings the block's values below 2^11, as far as f16 can hold
-  // 2^-power.  A barrier for all.
-  const auto common_power = [&](int32_t largest) {
-    largest = __reduce_max_sync(0xffffffffu, largest);
-    if (lane == 0) control.tops[warp] = largest;
-    __syncthreads();
+    uint32_t largest = 0;
 #pragma unroll
-    for (int w = 0; w < kBlockThreads / 32; ++w) largest = max(largest, control.tops[w]);
-    return max(largest - 24, -15);
-  };
-  // Multiplies the output so far.
-  const auto rescale = [&](float by) {
+    for (int k = 0; k < kWords; ++k) w[k] &= 0x7fff7fffu;
+    if (first_row + L::kTile > seen_max)
 #pragma unroll
-    for (int k = 0; k < D / 2; k += 16) {
-      uint32_t o[16];
-      tmem_load<16>(lanes + half * (D / 2) + k, o);
+      for (int k = 0; k < kWords; ++k)
+        if (first_row + (lane * kWords + k) / L::kGroups >= seen_max) w[k] = 0;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
-      tc::tmem_store16(lanes + half * (D / 2) + k, o);
+    for (int k = 0; k < kWords; ++k) largest = __vmaxu2(largest, w[k]);
+    const bool passes = (largest & 0xffffu) >= static_cast<uint32_t>(26 + power) << 10 ||
+                        (largest >> 16) >= static_cast<uint32_t>(29 + power) << 10;
+    if (!first && !__any_sync(0xffffffffu, passes)) return power;
+    int32_t field = 0;
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
+      const int32_t scale = w[k] >> 10 & 31, offset = w[k] >> 26;
+      field = max(field, max(scale < 31 ? scale + 3 : 0, offset < 31 ? offset : 0));
     }
-    tc::tmem_wait_store();
+    field = __reduce_max_sync(0xffffffffu, field);
+    return max(field - 24, first ? -15 : power);
   };
   const auto waits = [&](uint32_t barrier, uint32_t parity) {
     if (!wait(barrier, parity, abort)) {
@@ -422,7 +417,7 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
       const uint32_t slot = count % L::kStages;
       const int32_t first_row = (s.tile0 + i) * L::kTile;
       uint8_t *const stage = shared + L::kStageAt + slot * L::kStage;
-      bool large = false;
+      float change = 1.0f;  // of the output so far, with the values' power
       const uint32_t keys_at = base + (GROUP ? L::kOperandAt : L::kStageAt + slot * L::kStage);
       const uint32_t values_at = keys_at + L::kOperand;
       waits(shared_address(&control.landed[slot]), (count / L::kStages) & 1);
@@ -441,9 +436,11 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
           const float2 a = __half22float2(scales[0]), b = __half22float2(scales[L::kGroups]);
           reinterpret_cast<float4 *>(shared + L::kTableAt)[k] = make_float4(a.x, b.x, a.y, b.y);
         }
+        const int32_t next = tile_power(stage, first_row, s.seen_max, power, i == 0);
+        if (i > 0) change = __int_as_float((127 + power - next) << 23);
+        power = next;
         if (i > 0) waits(added, (count - 1) & 1);  // the last tile's values have been used
-        if (i == 0) power = common_power(largest_scales(stage, first_row, s.seen_max));
-        large = unpack_values(stage, first_row, s.seen_max, power);
+        unpack_values(stage, first_row, s.seen_max, power);
       } else {
         if (i > 0) waits(added, (count - 1) & 1);
         if (warp == 1 && i + 1 < tiles) feed(s, s.tile0 + i + 1, count + 1);  // into the stage that is free now
@@ -455,21 +452,7 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       before_sync();
-      if constexpr (GROUP == 0) {
-        __syncthreads();
-      } else if (__syncthreads_or(large)) {
-        // Values that pass 2^15 (or scales that are not finite): a new power.
-        const int32_t next = max(power, common_power(largest_scales(stage, first_row, s.seen_max)));
-        if (next != power) {
-          after_sync();
-          if (i > 0) rescale(__int_as_float((127 + power - next) << 23));
-          power = next;
-          unpack_values(stage, first_row, s.seen_max, power);
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          before_sync();
-          __syncthreads();
-        }
-      }
+      __syncthreads();
       after_sync();
       if (threadIdx.x == 0) {
 #pragma unroll
@@ -524,7 +507,7 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
       // The barrier also keeps the weights from the scores that others still read.
       before_sync();
       // (Also where best is NaN: top has to become NaN, since -inf stands for no rows.)
-      const bool raises = __syncthreads_or(!(fmaf(best, factor, -kMost) <= top));
+      const bool raises = __syncthreads_or(!(fmaf(best, factor, -kMost) <= top) || (GROUP != 0 && change != 1.0f));
       after_sync();
       if (raises) {
         stats[half * kBlockRows + row] = best;
@@ -534,7 +517,17 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
         const float keep = top == -INFINITY ? 0.0f : exp2_fast(top - next);
         top = next;
         sum *= keep;
-        if (i > 0 && __any_sync(0xffffffffu, keep != 1.0f)) rescale(keep);
+        if (i > 0 && __any_sync(0xffffffffu, keep * change != 1.0f)) {
+#pragma unroll
+          for (int k = 0; k < D / 2; k += 16) {
+            uint32_t o[16];
+            tmem_load<16>(lanes + half * (D / 2) + k, o);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * (keep * change));
+            tc::tmem_store16(lanes + half * (D / 2) + k, o);
+          }
+          tc::tmem_wait_store();
+        }
         __syncthreads();  // before the maxima are written over
       }
       const float shift = top == -INFINITY ? 0.0f : -top;
