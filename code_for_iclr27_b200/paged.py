@@ -183,9 +183,14 @@ class PagedCache:
             at = upload(np.asarray(entries, dtype=np.int64).T.copy(), self.device)
             self.tables.index_put_((at[0], at[1], at[2]), at[3].to(torch.int32))
 
+    def _slots(self, sequence: int) -> slice:
+        if not 0 <= sequence < self.sequences:
+            raise ValueError(f"the cache has sequences 0 to {self.sequences - 1}, not {sequence}")
+        return slice(sequence * self.heads, (sequence + 1) * self.heads)
+
     def release(self, sequence: int) -> None:
         """Return a sequence's pages; its slots become empty."""
-        slots = slice(sequence * self.heads, (sequence + 1) * self.heads)
+        slots = self._slots(sequence)
         for layer in self._held:
             for slot in range(slots.start, slots.stop):
                 self._free.extend(reversed(layer[slot]))
@@ -246,15 +251,31 @@ class PagedCache:
 
     def load(self, sequence: int, packed) -> None:
         """Put a request (kvcache.PackedCache) into a sequence, in place of what it held: the rows are already
-        rotated, so they are only stored (quantised where the pages are 4-bit)."""
+        rotated, so they are only stored (quantised where the pages are 4-bit).  Raises, with nothing changed, ValueError
+        for a request of another shape or type and MemoryError for one that the pages do not hold."""
         import torch
 
-        if len(packed.layers) != self.layers or packed.heads != self.heads:
+        slots = self._slots(sequence)
+        if len(packed.layers) != self.layers or any(len(layer.head_lens) != self.heads for layer in packed.layers):
             raise ValueError("packed cache has another number of layers or heads")
-        self.release(sequence)
-        slots = slice(sequence * self.heads, (sequence + 1) * self.heads)
+        types = (torch.float16, torch.bfloat16) if self.pages.key_scales is not None else (self.pages.keys.dtype,)
+        for layer in packed.layers:
+            if layer.keys.dtype not in types or layer.values.dtype != layer.keys.dtype:
+                raise ValueError(f"rows of {layer.keys.dtype} and {layer.values.dtype} into pages of {self.pages.keys.dtype}")
+            if layer.keys.shape != (sum(layer.head_lens), self.dim) or layer.values.shape != layer.keys.shape or (
+                    layer.positions.numel() != layer.keys.shape[0]):
+                raise ValueError("packed rows do not fit the head lengths or the cache's head dimension")
+            if any(t.device != self.lengths.device for t in (layer.keys, layer.values, layer.positions, layer.cumulative)):
+                raise ValueError("packed rows are on another device")
         rows = self.rows.copy()
         rows[:, slots] = [layer.head_lens for layer in packed.layers]
+        need = -(-rows[:, slots] // self.page_size)
+        free = len(self._free) + sum(len(pages) for layer in self._held for pages in layer[slots])
+        if int(need.max(initial=0)) > self.tables.shape[2]:
+            raise MemoryError(f"a slot would pass {self.tables.shape[2] * self.page_size} rows")
+        if int(need.sum()) > free:
+            raise MemoryError(f"{int(need.sum())} pages needed, {free} free without what the sequence holds")
+        self.release(sequence)
         self._hold(rows)
         self.rows[:] = rows
         self.prompt_rows[:, slots] = [layer.prompt_lens for layer in packed.layers]
@@ -270,7 +291,7 @@ class PagedCache:
         from .kvcache import PackedCache
 
         packed = PackedCache()
-        slots = slice(sequence * self.heads, (sequence + 1) * self.heads)
+        slots = self._slots(sequence)
         first = self.lengths.new_zeros(self.heads)
         for index in range(self.layers):
             lens = self.rows[index, slots]

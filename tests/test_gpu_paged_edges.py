@@ -272,3 +272,76 @@ def queries_of_shape(shape, seed, device):
     import torch
 
     return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16).to(device)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_load_that_fails_changes_nothing(cuda, bits):
+    """Too many rows for the pages or for a slot, another dimension, type, number of heads or of layers: the sequence
+    keeps what it held."""
+    import torch
+
+    from code_for_iclr27_b200.kvcache import PackedCache
+    from code_for_iclr27_b200.paged import PagedCache
+    from test_gpu_arena import make_packed
+
+    packed = make_packed(cuda, seed=1)
+    cache = PagedCache(3, 2, 4, 128, 170, cuda, bits=bits, page_size=64, max_rows=1024)
+    cache.load(1, packed)
+
+    def state():
+        back = cache.to_packed(1)
+        return ([t for layer in back.layers for t in (layer.keys, layer.values, layer.positions, layer.cumulative)],
+                [(layer.head_lens, layer.prompt_lens) for layer in back.layers], cache.rows.tolist(),
+                cache.prompt_rows.tolist(), cache.free_pages(), cache.lengths.tolist())
+
+    before = state()
+
+    def made(rows=64, dim=128, dtype=torch.bfloat16, heads=4, layers=3, values=None):
+        other = PackedCache()
+        for _ in range(layers):
+            keys = torch.zeros(heads * rows, dim, dtype=dtype, device=cuda)
+            other.add_layer(keys, keys.clone() if values is None else values(keys), torch.zeros(heads * rows, device=cuda),
+                            [rows] * heads, [0] * heads)
+        return other
+
+    wrong = [(MemoryError, made(rows=1000)), (MemoryError, made(rows=1100)), (ValueError, made(dim=64)), (ValueError, made(heads=3)),
+             (ValueError, made(layers=2)), (ValueError, made(dtype=torch.float32)), (ValueError, PackedCache()),
+             (ValueError, made(values=lambda k: k[:-1])), (ValueError, made(values=lambda k: k.half()))]
+    elsewhere = made()
+    elsewhere.layers[2].values = elsewhere.layers[2].values.cpu()
+    wrong.append((ValueError, elsewhere))
+    if bits == 16:
+        wrong.append((ValueError, made(dtype=torch.float16)))
+    for error, other in wrong:
+        with pytest.raises(error):
+            cache.load(1, other)
+        now = state()
+        assert now[1:] == before[1:]
+        assert all(torch.equal(a, b) for a, b in zip(now[0], before[0]))
+    for sequence in (-1, 2):
+        for call in (lambda: cache.load(sequence, packed), lambda: cache.release(sequence), lambda: cache.to_packed(sequence)):
+            with pytest.raises(ValueError):
+                call()
+    # What the sequence holds counts as free: a request that fits only in its place is taken.
+    taken = cache.free_pages()
+    cache.load(1, made(rows=64 * ((170 - 2) // 12)))
+    assert taken < 170 // 2 + 60 and cache.free_pages() == 170 - 12 * ((170 - 2) // 12)
+    cache.check_flags()
+
+
+def test_load_of_a_type_that_4_bit_rows_take(cuda):
+    """float16 rows into the 4-bit pages of a bfloat16 cache, as before."""
+    import torch
+
+    from code_for_iclr27_b200.kvcache import PackedCache
+    from code_for_iclr27_b200.paged import PagedCache
+
+    packed = PackedCache()
+    rows = torch.randn(2 * 50, 64, generator=torch.Generator().manual_seed(0)).half().to(cuda)
+    packed.add_layer(rows, rows * 2, torch.arange(100, dtype=torch.float32, device=cuda), [50, 50], [10, 20])
+    cache = PagedCache(1, 1, 2, 64, 8, cuda, bits=4, group=32, page_size=16)
+    cache.load(0, packed)
+    back = cache.to_packed(0, torch.float32).layers[0]
+    step = (rows.float().unflatten(-1, (2, 32)).amax(-1) - rows.float().unflatten(-1, (2, 32)).amin(-1)) / 15
+    assert ((back.keys - rows.float()).abs().unflatten(-1, (2, 32)).amax(-1) <= 0.6 * step).all()
+    cache.check_flags()
