@@ -149,6 +149,7 @@ class PagedCache:
         self.flag = torch.zeros(1, dtype=torch.int32, device=self.device)
         self.rows = np.zeros((self.layers, slots), dtype=np.int64)  # host mirror of the lengths
         self.prompt_rows = np.zeros((self.layers, slots), dtype=np.int64)
+        self.seen_tokens = np.zeros(self.sequences, dtype=np.int64)  # as PackedCache.seen_tokens, a step's tokens added
         self._free: List[int] = list(range(int(pages) - 1, -1, -1))
         self._held: List[List[List[int]]] = [[[] for _ in range(slots)] for _ in range(self.layers)]
         self._workspaces = {}
@@ -197,6 +198,7 @@ class PagedCache:
                 layer[slot] = []
         self.rows[:, slots] = 0
         self.prompt_rows[:, slots] = 0
+        self.seen_tokens[sequence] = 0
         self.lengths[:, slots] = 0
 
     def check_flags(self) -> None:
@@ -220,6 +222,7 @@ class PagedCache:
         per_slot = np.repeat(counts, self.heads)
         self._hold(self.rows + per_slot)
         self.rows += per_slot
+        self.seen_tokens += counts
         starts = np.concatenate(([0], np.cumsum(counts)))
         both = upload(np.concatenate((starts, per_slot)).astype(np.int32), self.device)
         self.token_starts = both[:self.sequences + 1]
@@ -279,6 +282,7 @@ class PagedCache:
         self._hold(rows)
         self.rows[:] = rows
         self.prompt_rows[:, slots] = [layer.prompt_lens for layer in packed.layers]
+        self.seen_tokens[sequence] = packed.seen_tokens
         self.lengths[:, slots] = upload(rows[:, slots].astype(np.int32), self.device)
         for index, layer in enumerate(packed.layers):
             # Each head's rows are the new tokens of a one-head sequence of their own.
@@ -287,11 +291,11 @@ class PagedCache:
                          self.flag)
 
     def to_packed(self, sequence: int, dtype=None):
-        """A sequence's rows as a kvcache.PackedCache of `dtype` (the cache's by default)."""
+        """A sequence's rows (and its count of seen tokens) as a kvcache.PackedCache of `dtype` (the cache's by default)."""
         from .kvcache import PackedCache
 
-        packed = PackedCache()
         slots = self._slots(sequence)
+        packed = PackedCache(seen_tokens=int(self.seen_tokens[sequence]))
         first = self.lengths.new_zeros(self.heads)
         for index in range(self.layers):
             lens = self.rows[index, slots]

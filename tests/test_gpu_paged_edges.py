@@ -345,3 +345,22 @@ def test_load_of_a_type_that_4_bit_rows_take(cuda):
     step = (rows.float().unflatten(-1, (2, 32)).amax(-1) - rows.float().unflatten(-1, (2, 32)).amin(-1)) / 15
     assert ((back.keys - rows.float()).abs().unflatten(-1, (2, 32)).amax(-1) <= 0.6 * step).all()
     cache.check_flags()
+
+
+def test_tokens_seen_come_back(cuda):
+    """A request's count of seen tokens goes into the pages and back with it, a step's tokens added."""
+    from code_for_iclr27_b200.arena import ArenaCache
+    from code_for_iclr27_b200.paged import PagedCache
+    from test_gpu_arena import make_packed
+
+    packed = [make_packed(cuda, seed=s) for s in (1, 2)]
+    packed[1].seen_tokens = 5000
+    cache = PagedCache(3, 2, 4, 128, 400, cuda, bits=4, page_size=64, max_rows=2048)
+    for s in range(2):
+        cache.load(s, packed[s])
+    assert [cache.to_packed(s).seen_tokens for s in range(2)] == [packed[0].seen_tokens, 5000]
+    cache.advance([1, 7])
+    assert [cache.to_packed(s).seen_tokens for s in range(2)] == [packed[0].seen_tokens + 1, 5007]
+    assert ArenaCache.from_packed(cache.to_packed(1), margin=8).seen_tokens == 5007
+    cache.release(1)
+    assert cache.to_packed(1).seen_tokens == 0 and cache.to_packed(0).seen_tokens == packed[0].seen_tokens + 1
