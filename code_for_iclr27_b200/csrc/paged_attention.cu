@@ -152,6 +152,7 @@ struct Control {
   Walk<ROWS, kTile> walk;
   int32_t abort;
   int32_t arrived[2];
+  uint8_t gone[2 * kWarps];  // of a stage's tile: bit h set where the page of its rows 16 h .. does not exist
   Segment pending[2];
   Segment segments[2];  // this one and the next; slot -1 ends them
 };
@@ -443,27 +444,33 @@ struct Consumer {
     }
   }
 
+  // With MASKED, rows that a query does not see are left out, and so are the 16
+  // rows of half h where bit h of `gone` is set.
   template <bool MASKED>
   __device__ __forceinline__ void tile(uint8_t *stage, const uint8_t *query_at, const float *group_sums, int lane,
-                                       int32_t first_row, int32_t seen_max, const int32_t *seen_by) {
+                                       int32_t first_row, int32_t seen_max, const int32_t *seen_by, uint32_t gone) {
     float s[2][NT][4];
     scores(stage, query_at, group_sums, lane, s);
+    // Rows that are gone count as rows beyond every slot's length.
+    constexpr int32_t kFar = INT32_MAX - 2 * kTile;
+    const int32_t first[2] = {gone & 1 ? kFar : first_row, gone & 2 ? kFar : first_row};
     if constexpr (MASKED) {
       const int g = lane >> 2;
-      const int row = first_row + (GROUP == 0 ? g : g ^ ((g >> 1) & 1));
+      const int row = GROUP == 0 ? g : g ^ ((g >> 1) & 1);
 #pragma unroll
       for (int half = 0; half < 2; ++half)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (row + half * 16 + (i < 2 ? 0 : 8) >= seen_by[nt * 8 + 2 * (lane & 3) + (i & 1)]) s[half][nt][i] = -INFINITY;
+            if (first[half] + row + half * 16 + (i < 2 ? 0 : 8) >= seen_by[nt * 8 + 2 * (lane & 3) + (i & 1)])
+              s[half][nt][i] = -INFINITY;
     }
     uint32_t largest = 0;
     if constexpr (GROUP != 0) {
-      // What lies beyond every query's rows (or, past a page of 16, was never
-      // copied) may be anything, and must not raise `lift`.
-      if (!MASKED || first_row + lane < seen_max) largest = largest_scale(stage, lane);
+      // What lies beyond every query's rows (or was never copied) may be anything,
+      // and must not raise `lift`.
+      if (!MASKED || (lane < 16 ? first[0] : first[1]) + lane < seen_max) largest = largest_scale(stage, lane);
     }
     bool raises = largest > plain_scale();
     float best[NT][2];
@@ -490,7 +497,7 @@ struct Consumer {
       }
     if constexpr (MASKED && GROUP == 0) {
       // What lies beyond every query's rows may be NaN, and 0 NaN is NaN.
-      if (first_row + lane >= seen_max)
+      if ((lane < 16 ? first[0] : first[1]) + lane >= seen_max)
 #pragma unroll
         for (int c = 0; c < D / 8; ++c)
           *reinterpret_cast<uint4 *>(stage + L::kCodes + (c >> 3) * (kTile * 128) + lane * 128 + (c & 7) * 16) =
@@ -498,7 +505,7 @@ struct Consumer {
       __syncwarp();
     }
 #pragma unroll
-    for (int half = 0; half < 2; ++half) values<MASKED>(stage, half, lane, s[half], first_row, seen_by);
+    for (int half = 0; half < 2; ++half) values<MASKED>(stage, half, lane, s[half], first[half], seen_by);
   }
 };
 
@@ -522,6 +529,7 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
     for (int i = 0; i < L::kStages; ++i) tc::init_barrier(shared_address(&control.landed[i]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     *abort = 0;
+    for (int i = 0; i < 2 * kWarps; ++i) control.gone[i] = 0;
   }
   int64_t share;
   if (!begin<kThreads, kMinTiles, kCrossing>(p, &control.sums[0][0], share, control.walk, control.segments[0])) return;
@@ -540,27 +548,36 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
   constexpr float kLeastFactor = 1e-37f;
   int pieces = 0;
   uint32_t phases = 0;  // of this warp's stages, a bit each
+  // Set where this warp has met a page that does not exist in the segment: only
+  // then is control.gone read and written.
+  constexpr uint32_t kLost = 0x100;
 
   for (int number = 0;; ++number) {
     const Segment &s = control.segments[number & 1];
     if (s.slot < 0) break;
     // Warp w takes tiles w, w + kWarps, .. of the stretch, and moves them into
-    // its own stages.  Lane i knows the page(s) of its tile number 32 k + i.
+    // its own stages.  Lane i knows the page(s) of its tile number 32 k + i; -1
+    // where the table names none, whose rows are left out.
     const int32_t tile0 = s.tile0 + warp, seen_min = s.seen_min, seen_max = s.seen_max;
     const int32_t own = max((s.tile1 - tile0 + kWarps - 1) / kWarps, 0);
     int32_t page0 = 0, page1 = 0;
+    if (phases & kLost) {
+      if (lane < L::kDepth) control.gone[warp * L::kDepth + lane] = 0;
+      phases &= ~kLost;
+      __syncwarp();
+    }
     const auto look_up = [&](int32_t n) {
       const int32_t *entries = p.table + static_cast<int64_t>(s.slot) * p.table_stride;
       const int32_t row = (tile0 + (n + lane) * kWarps) * kTile;
       if (n + lane < own) {
         page0 = entries[row >> p.pages.page_shift];
         if (p.pages.page_size == 16 && row + 16 < seen_max) page1 = entries[(row + 16) >> p.pages.page_shift];
-        if (static_cast<uint32_t>(page0) >= static_cast<uint32_t>(p.pages.pages) ||
-            static_cast<uint32_t>(page1) >= static_cast<uint32_t>(p.pages.pages)) {
-          page0 = page1 = 0;
-          atomicOr(p.flag, kFlagRow);
-        }
+        else page1 = 0;
+        if (static_cast<uint32_t>(page0) >= static_cast<uint32_t>(p.pages.pages)) page0 = -1;
+        if (static_cast<uint32_t>(page1) >= static_cast<uint32_t>(p.pages.pages)) page1 = -1;
+        if ((page0 | page1) < 0) atomicOr(p.flag, kFlagRow);
       }
+      if (__any_sync(0xffffffffu, n + lane < own && (page0 | page1) < 0)) phases |= kLost;
     };
     const auto feed = [&](int32_t n) {
       if ((n & 31) == 0) look_up(n);
@@ -571,8 +588,15 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
       const bool halves = p.pages.page_size == 16;
       const int rows = halves ? 16 : kTile;
       const int copies = halves && row + 16 < seen_max ? 2 : 1;  // pages that the tile's visible rows lie in
-      tc::expect_bytes(barrier, copies * rows * (L::kStage / kTile));
+      int there = copies;
+      if (phases & kLost) {
+        const int gone0 = page0 < 0, gone1 = copies == 2 && page1 < 0;
+        control.gone[slot] = gone0 && !halves ? 3 : gone0 | gone1 << 1;
+        there -= gone0 + gone1;
+      }
+      tc::expect_bytes(barrier, there * rows * (L::kStage / kTile));
       for (int part = 0; part < copies; ++part) {
+        if ((part ? page1 : page0) < 0) continue;
         const int64_t y = static_cast<int64_t>(part ? page1 : page0) * p.pages.page_size +
                           (row & (p.pages.page_size - 1));
 #pragma unroll
@@ -681,17 +705,18 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
       uint8_t *const at = shared + (warp * L::kDepth + slot) * L::kStage;
       const int32_t first_row = (tile0 + n * kWarps) * kTile;
       const bool landed = __all_sync(0xffffffffu, wait(barrier, (phases >> slot) & 1, abort));
+      const uint32_t gone = phases & kLost ? control.gone[warp * L::kDepth + slot] : 0;
       if (!landed) {
         // Given up: nothing more is computed, but every barrier is still met,
         // and the copy in flight gets its time to land.
         if (lane == 0) atomicOr(p.flag, kFlagTimeout);
         *abort = 1;
         tc::wait_phase(barrier, (phases >> slot) & 1, nullptr);
-      } else if (first_row + kTile > seen_min) {
-        c.template tile<true>(at, query_at, group_sums, lane, first_row, seen_max, seen_by);
+      } else if (first_row + kTile > seen_min || gone) {
+        c.template tile<true>(at, query_at, group_sums, lane, first_row, seen_max, seen_by, gone);
         if constexpr (GROUP == 0) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       } else {
-        c.template tile<false>(at, query_at, group_sums, lane, first_row, seen_max, seen_by);
+        c.template tile<false>(at, query_at, group_sums, lane, first_row, seen_max, seen_by, 0);
       }
       phases ^= 1u << slot;
       __syncwarp();

@@ -75,6 +75,10 @@ struct TcLayout {
 template <int TILE>
 struct TcControl {
   uint64_t landed[3], scored, added;
+  // Of tile number n, at n % 4 (more than there are stages: a later tile is fed
+  // before the scores are masked): a bit for each row that lies beyond every
+  // query's rows, or in a page that does not exist.
+  uint64_t absent[4];
   int64_t sums[2][kBlockThreads / 32];
   Walk<kBlockRows, TILE> walk;
   uint32_t columns;
@@ -240,16 +244,24 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
     // Pages that hold visible rows of the tile; others may not exist.
     const int parts = min(L::kTile / rows, (s.seen_max - first + rows - 1) >> min(p.pages.page_shift, L::kTile == 64 ? 6 : 5));
     constexpr int kKinds = GROUP ? 4 : 2 * (D / 64);
-    if (lane == 0) tc::expect_bytes(barrier, parts * rows * (L::kStage / L::kTile));
-    __syncwarp();
     const int part = lane / kKinds, kind = lane % kKinds;
-    if (part < parts) {
-      const int32_t at = first + part * rows;
-      int32_t page = p.table[static_cast<int64_t>(s.slot) * p.table_stride + (at >> p.pages.page_shift)];
-      if (page < 0 || page >= p.pages.pages) {
-        page = 0;
+    const int32_t at = first + part * rows;
+    int32_t page = -1;
+    if (part < parts) page = p.table[static_cast<int64_t>(s.slot) * p.table_stride + (at >> p.pages.page_shift)];
+    const bool there = page >= 0 && page < p.pages.pages;
+    const uint32_t found = __ballot_sync(0xffffffffu, there && kind == 0);
+    if (lane == 0) {
+      uint64_t absent = s.seen_max - first < L::kTile ? ~uint64_t{0} << (s.seen_max - first) : 0;
+      if (__popc(found) < parts) {
+        for (int i = 0; i < parts; ++i)
+          if (!(found >> (i * kKinds) & 1)) absent |= (~uint64_t{0} >> (64 - rows)) << (i * rows);
         atomicOr(p.flag, kFlagRow);
       }
+      control.absent[n & 3] = absent;
+      tc::expect_bytes(barrier, __popc(found) * rows * (L::kStage / L::kTile));
+    }
+    __syncwarp();
+    if (there) {
       const int64_t y = static_cast<int64_t>(page) * p.pages.page_size + (at & (p.pages.page_size - 1));
       if constexpr (GROUP == 0) {
         const int side = kind / (D / 64), box = kind % (D / 64);
@@ -270,10 +282,10 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
     __syncwarp();
   };
   // Unpacking values: a thread keeps its chunk of 8 channels, and takes every
-  // (threads / chunks)th row.  Rows from `seen_max` on may hold anything, and
-  // 0 NaN is NaN.
+  // (threads / chunks)th row.  `absent` (a bit for each of the tile's rows): rows
+  // beyond every query's, or without a page, may hold anything, and 0 NaN is NaN.
   constexpr int kChunks = D / 8, kStep = kBlockThreads / kChunks;
-  const auto unpack_values = [&](const uint8_t *stage, int32_t first_row, int32_t seen_max, int32_t power) {
+  const auto unpack_values = [&](const uint8_t *stage, uint64_t absent, int32_t power) {
     const int c = threadIdx.x % kChunks;
     const uint8_t *value_stage = stage + L::kCodes + L::kScales;
     const __half2 down = __half2half2(__ushort_as_half(static_cast<unsigned short>((15 - power) << 10)));
@@ -286,9 +298,15 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
       const __half2 scale = __low2half2(pair), offset = __high2half2(pair);
 #pragma unroll
       for (int k = 0; k < 4; ++k) n[k] = __hfma2(n[k], scale, offset);
-      if (first_row + r >= seen_max) n[0] = n[1] = n[2] = n[3] = __float2half2_rn(0.0f);
       *reinterpret_cast<uint4 *>(shared + L::kOperandAt + L::kOperand + chunk_at(r, c, L::kTile)) =
           *reinterpret_cast<uint4 *>(n);
+    }
+    if (absent != 0) {
+#pragma unroll 1
+      for (int r = threadIdx.x / kChunks; r < L::kTile; r += kStep)
+        if (absent >> r & 1)
+          *reinterpret_cast<uint4 *>(shared + L::kOperandAt + L::kOperand + chunk_at(r, c, L::kTile)) =
+              make_uint4(0, 0, 0, 0);
     }
   };
   // The power for a tile's values, found by every warp for itself: a lane holds a
@@ -297,7 +315,7 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
   // the power stays while that is at most 2^(15 + power), and brings it below
   // 2^(11 + power) otherwise (as far as f16 holds 2^-power).  Pairs that are not
   // finite reach their own rows, whatever the power.
-  const auto tile_power = [&](const uint8_t *stage, int32_t first_row, int32_t seen_max, int32_t power, bool first) {
+  const auto tile_power = [&](const uint8_t *stage, uint64_t absent, int32_t power, bool first) {
     constexpr int kWords = L::kTile * L::kGroups / 32;
     uint32_t w[kWords];
     const uint8_t *from = stage + 2 * L::kCodes + L::kScales + lane * kWords * 4;
@@ -311,10 +329,10 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
     uint32_t largest = 0;
 #pragma unroll
     for (int k = 0; k < kWords; ++k) w[k] &= 0x7fff7fffu;
-    if (first_row + L::kTile > seen_max)
+    if (absent != 0)
 #pragma unroll
       for (int k = 0; k < kWords; ++k)
-        if (first_row + (lane * kWords + k) / L::kGroups >= seen_max) w[k] = 0;
+        if (absent >> ((lane * kWords + k) / L::kGroups) & 1) w[k] = 0;
 #pragma unroll
     for (int k = 0; k < kWords; ++k) largest = __vmaxu2(largest, w[k]);
     const bool passes = (largest & 0xffffu) >= static_cast<uint32_t>(26 + power) << 10 ||
@@ -421,6 +439,7 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
       const uint32_t keys_at = base + (GROUP ? L::kOperandAt : L::kStageAt + slot * L::kStage);
       const uint32_t values_at = keys_at + L::kOperand;
       waits(shared_address(&control.landed[slot]), (count / L::kStages) & 1);
+      const auto absent_rows = [&] { return *const_cast<volatile uint64_t *>(&control.absent[count & 3]); };
       if constexpr (GROUP != 0) {
         const int c = threadIdx.x % kChunks;
         uint8_t *const operands = shared + L::kOperandAt;
@@ -436,17 +455,19 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
           const float2 a = __half22float2(scales[0]), b = __half22float2(scales[L::kGroups]);
           reinterpret_cast<float4 *>(shared + L::kTableAt)[k] = make_float4(a.x, b.x, a.y, b.y);
         }
-        const int32_t next = tile_power(stage, first_row, s.seen_max, power, i == 0);
+        const uint64_t absent = absent_rows();
+        const int32_t next = tile_power(stage, absent, power, i == 0);
         if (i > 0) change = __int_as_float((127 + power - next) << 23);
         power = next;
         if (i > 0) waits(added, (count - 1) & 1);  // the last tile's values have been used
-        unpack_values(stage, first_row, s.seen_max, power);
+        unpack_values(stage, absent, power);
       } else {
         if (i > 0) waits(added, (count - 1) & 1);
         if (warp == 1 && i + 1 < tiles) feed(s, s.tile0 + i + 1, count + 1);  // into the stage that is free now
-        if (first_row + L::kTile > s.seen_max)
+        const uint64_t absent = absent_rows();
+        if (absent != 0)
           for (int k = threadIdx.x; k < L::kTile * (D / 8); k += kBlockThreads)
-            if (first_row + k % L::kTile >= s.seen_max)
+            if (absent >> (k % L::kTile) & 1)
               *reinterpret_cast<uint4 *>(stage + L::kOperand + chunk_at(k % L::kTile, k / L::kTile, L::kTile)) =
                   make_uint4(0, 0, 0, 0);
       }
@@ -493,12 +514,13 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
           }
         }
       }
-      if (first_row + L::kTile > s.seen_min) {
+      if (const uint64_t absent = absent_rows(); first_row + L::kTile > s.seen_min || absent != 0) {
         const int32_t visible = seen - first_row - half * L::kHalf;
+        const uint32_t hidden = static_cast<uint32_t>(absent >> (half * L::kHalf));
 #pragma unroll
         for (int k = 0; k < L::kHalf / 2; ++k) {
-          if (2 * k >= visible) x[k].x = -INFINITY;
-          if (2 * k + 1 >= visible) x[k].y = -INFINITY;
+          if (2 * k >= visible || (hidden >> (2 * k) & 1)) x[k].x = -INFINITY;
+          if (2 * k + 1 >= visible || (hidden >> (2 * k + 1) & 1)) x[k].y = -INFINITY;
         }
       }
       float best = max_nan(x[0].x, x[0].y);

@@ -563,10 +563,11 @@ int lrk_paged_append(const lrk_pages *pages, const int32_t *table, int64_t table
  * r <= lengths[slot] - n_s + i, without it every row below lengths[slot].
  * out [tokens, query_heads, dimension] of dtype = softmax(scale q k) v, lse
  * f32 [tokens, query_heads] = log sum exp(scale q k); a query without a
- * visible row gives 0 and -inf.  What lies in pages beyond a slot's length is
- * never used.  A NaN key reaches the queries that see its row and no other; a
- * value that is not finite may, in a call of several queries a sequence, also
- * reach those of the slot's queries that do not see its row (0 times NaN).
+ * visible row gives 0 and -inf.  Rows whose table entry names no page are left
+ * out.  What lies in pages beyond a slot's length is never used.  A NaN key
+ * reaches the queries that see its row and no other; a value that is not finite
+ * may, in a call of several queries a sequence, also reach those of the slot's
+ * queries that do not see its row (0 times NaN).
  * 16-bit pages and queries share one type.  Sums and softmax statistics are float32;
  * weights are rounded once to f16 (4-bit and f16 rows) or bf16.
  * workspace: lrk_paged_attention_workspace_bytes() bytes, 16-byte aligned,

@@ -364,3 +364,31 @@ def test_tokens_seen_come_back(cuda):
     assert ArenaCache.from_packed(cache.to_packed(1), margin=8).seen_tokens == 5007
     cache.release(1)
     assert cache.to_packed(1).seen_tokens == 0 and cache.to_packed(0).seen_tokens == packed[0].seen_tokens + 1
+
+
+@pytest.mark.parametrize("bits,dtype,dim,group", FORMATS)
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("tokens,groups", [(1, 4), (3, 4), (5, 6), (70, 1)])
+def test_rows_whose_page_does_not_exist_are_left_out(cuda, bits, dtype, dim, group, page, tokens, groups):
+    """A page id outside the pages takes that page's rows out of the slot, and nothing else; the flag says so."""
+    import torch
+
+    case = Case(cuda, bits, dtype, dim, group, page, 2, [300, 75, 150, 16, 40, 600], seed=page)
+    counts = [tokens] * 3
+    queries = queries_of(case, counts, groups)
+    good, good_lse = case.attend(queries, counts)
+    compare(case, queries, counts, good, good_lse)
+    absent = {}
+    for slot, at, entry in ((0, 0, -1), (0, 1, 2 ** 30), (1, 75 // page, -2 ** 31), (2, 1, 2 ** 31 - 1), (3, 0, -5),
+                            (5, 300 // page, 2 ** 20), (5, 599 // page, -1)):
+        case.table[slot, at] = entry
+        rows = np.arange(at * page, (at + 1) * page)
+        absent[slot] = np.union1d(absent.get(slot, np.zeros(0, dtype=int)), rows)
+    out, lse = case.attend(queries, counts)
+    compare(case, queries, counts, out, lse, absent=absent, flag=1)
+    again, again_lse = case.attend(queries, counts)
+    assert torch.equal(out, again) and torch.equal(lse, again_lse)
+    case.flag.zero_()
+    # The untouched slot of the last sequence is as it was.
+    at = slice(2 * tokens, 3 * tokens)
+    assert torch.allclose(out[at, :groups].float(), good[at, :groups].float(), rtol=2 ** -7, atol=1e-6)
