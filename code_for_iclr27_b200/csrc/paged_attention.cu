@@ -532,7 +532,7 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
     for (int i = 0; i < 2 * kWarps; ++i) control.gone[i] = 0;
   }
   int64_t share;
-  if (!begin<kThreads, kMinTiles, kCrossing>(p, &control.sums[0][0], share, control.walk, control.segments[0])) return;
+  if (!begin<D, kThreads, kMinTiles, kCrossing>(p, &control.sums[0][0], share, control.walk, control.segments[0])) return;
 
   Consumer<T, D, GROUP, NT> c;
   float *group_sums = reinterpret_cast<float *>(shared + L::kSumsAt);

@@ -176,9 +176,26 @@ struct Walk {
   }
 };
 
+// Tokens of no sequence (before the first one's `start`, from the last one's
+// `stop` on) see nothing: one block writes their outputs.  Out of line: hardly any
+// call needs it, and every block would fetch its instructions.
+template <int D, int THREADS>
+__device__ __noinline__ void fill_lost(const AttentionParam &p, int32_t start, int32_t stop) {
+  if (threadIdx.x == 0) atomicOr(p.flag, kFlagRow);
+  const int32_t before = min(max(start, 0), p.tokens), after = min(max(stop, 0), p.tokens);
+  const int64_t rows = static_cast<int64_t>(before + p.tokens - after) * p.heads * p.groups;
+  for (int64_t i = threadIdx.x; i < rows * (D / 8); i += THREADS) {
+    int64_t row = i / (D / 8);
+    if (row >= static_cast<int64_t>(before) * p.heads * p.groups)
+      row += static_cast<int64_t>(after - before) * p.heads * p.groups;
+    static_cast<uint4 *>(p.out)[row * (D / 8) + i % (D / 8)] = make_uint4(0, 0, 0, 0);
+    if (i % (D / 8) == 0) p.lse[row] = -INFINITY;
+  }
+}
+
 // A block's share of the work and its first segment; false for a block without
 // any.  sums: 2 x THREADS / 32 shared words.  Ends with a barrier.
-template <int THREADS, int MIN_TILES, int CROSSING, int ROWS, int TILE>
+template <int D, int THREADS, int MIN_TILES, int CROSSING, int ROWS, int TILE>
 __device__ __forceinline__ bool begin(const AttentionParam &p, int64_t *sums, int64_t &share,
                                       Walk<ROWS, TILE> &of_block, Segment &segment) {
   constexpr int kWarps = THREADS / 32;
@@ -192,7 +209,8 @@ __device__ __forceinline__ bool begin(const AttentionParam &p, int64_t *sums, in
     slot_work<ROWS, TILE>(p, i, s, units);
     units_sum += units;
     tiles_sum += static_cast<int64_t>(units) * s.unit_tiles;
-    if (blockIdx.x == 0 && p.lengths[i] > p.capacity) atomicOr(p.flag, kFlagRow);
+    if (blockIdx.x == 0 && (p.lengths[i] != s.length || p.token_starts[s.sequence + 1] < p.token_starts[s.sequence]))
+      atomicOr(p.flag, kFlagRow);  // a length that is negative or beyond the table, or starts that descend
   }
 #pragma unroll
   for (int step = 16; step > 0; step >>= 1) {
@@ -204,6 +222,10 @@ __device__ __forceinline__ bool begin(const AttentionParam &p, int64_t *sums, in
     sums[kWarps + warp] = units_sum;
   }
   __syncthreads();
+  if (blockIdx.x == gridDim.x - 1) {  // it has the least to do
+    const int32_t start = p.token_starts[0], stop = p.token_starts[p.by_heads(p.slots)];
+    if (start != 0 || stop != p.tokens) fill_lost<D, THREADS>(p, start, stop);
+  }
   tiles_sum = units_sum = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {

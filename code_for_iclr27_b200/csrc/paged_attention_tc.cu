@@ -207,7 +207,7 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
     *abort = 0;
   }
   int64_t share;
-  if (!begin<kBlockThreads, kLeastTiles, kUnitCrossing>(p, &control.sums[0][0], share, control.walk, control.segment)) return;
+  if (!begin<D, kBlockThreads, kLeastTiles, kUnitCrossing>(p, &control.sums[0][0], share, control.walk, control.segment)) return;
   // The instructions on tensor memory want their whole warp: lanes that a wait or
   // a branch held apart are brought together before each (__syncwarp).
   __syncwarp();

@@ -514,7 +514,8 @@ int lrk_arena_evict(const lrk_arena *arena, const int64_t *heads, const float *r
  * over it (src/lazy_recall/attention.py:15-35).
  *
  * The operators OR bits into *flag (device, required): 1 a length, row or
- * page id outside the table or the pages (that row is not touched), 2 a
+ * page id outside the table or the pages (that row is not touched; a negative
+ * length counts as 0) or a token of no sequence, 2 a
  * position outside the rotary table (that token's keys and queries are not
  * written), 4 a bounded wait inside a kernel ran out. */
 typedef struct lrk_pages {
@@ -563,11 +564,11 @@ int lrk_paged_append(const lrk_pages *pages, const int32_t *table, int64_t table
  * r <= lengths[slot] - n_s + i, without it every row below lengths[slot].
  * out [tokens, query_heads, dimension] of dtype = softmax(scale q k) v, lse
  * f32 [tokens, query_heads] = log sum exp(scale q k); a query without a
- * visible row gives 0 and -inf.  Rows whose table entry names no page are left
- * out.  What lies in pages beyond a slot's length is never used.  A NaN key
- * reaches the queries that see its row and no other; a value that is not finite
- * may, in a call of several queries a sequence, also reach those of the slot's
- * queries that do not see its row (0 times NaN).
+ * visible row, or of no sequence, gives 0 and -inf.  Rows whose table entry
+ * names no page are left out.  What lies in pages beyond a slot's length is never
+ * used.  A NaN key reaches the queries that see its row and no other; a value
+ * that is not finite may, in a call of several queries a sequence, also reach
+ * those of the slot's queries that do not see its row (0 times NaN).
  * 16-bit pages and queries share one type.  Sums and softmax statistics are float32;
  * weights are rounded once to f16 (4-bit and f16 rows) or bf16.
  * workspace: lrk_paged_attention_workspace_bytes() bytes, 16-byte aligned,

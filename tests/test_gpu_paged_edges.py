@@ -392,3 +392,56 @@ def test_rows_whose_page_does_not_exist_are_left_out(cuda, bits, dtype, dim, gro
     # The untouched slot of the last sequence is as it was.
     at = slice(2 * tokens, 3 * tokens)
     assert torch.allclose(out[at, :groups].float(), good[at, :groups].float(), rtol=2 ** -7, atol=1e-6)
+
+
+def fill_free_memory(device, sizes):
+    """NaN in the memory that outputs of these sizes (bytes) are given next."""
+    import torch
+
+    torch.cuda.synchronize()
+    held = [torch.full((size,), 0xff, dtype=torch.uint8, device=device) for size in sizes for _ in range(4)]
+    del held
+
+
+@pytest.mark.parametrize("bits,dtype,dim,group", [(16, "bf16", 128, 0), (4, "f16", 128, 64), (4, "bf16", 64, 32)])
+@pytest.mark.parametrize("groups", [1, 5, 40])
+@pytest.mark.parametrize("starts", [[2, 3, 5], [0, 0, 0], [8, 8, 8], [0, 4, 6], [1, 1, 8], [-3, 2, 8], [0, 3, 100]])
+def test_tokens_of_no_sequence(cuda, bits, dtype, dim, group, groups, starts):
+    """Eight tokens, some of them in no sequence: those see nothing (0 and -inf), the flag is set, the others are
+    computed."""
+    import torch
+
+    from code_for_iclr27_b200.paged import attention_workspace, paged_attention
+
+    case = Case(cuda, bits, dtype, dim, group, 32, 2, [100, 40, 64, 9], seed=3)
+    queries = queries_of(case, [8], groups)
+    fill_free_memory(cuda, [queries.numel() * 2, queries.shape[0] * queries.shape[1] * 4])
+    out, lse = paged_attention(case.pages, case.table, case.lengths, queries,
+                               torch.tensor(starts, dtype=torch.int32, device=cuda), attention_workspace(cuda), case.flag)
+    assert int(case.flag.item()) == 1
+    case.flag.zero_()
+    inside = [min(max(x, 0), 8) for x in starts]
+    lost = [t for t in range(8) if not inside[0] <= t < inside[2]]
+    assert (out[lost] == 0).all() and torch.isneginf(lse[lost]).all()
+    counts = [inside[1] - inside[0], inside[2] - inside[1]]
+    at = slice(inside[0], inside[2])
+    compare(case, queries[at], counts, out[at], lse[at])
+
+
+def test_starts_that_descend_and_negative_lengths_are_flagged(cuda):
+    import torch
+
+    from code_for_iclr27_b200.paged import attention_workspace, paged_attention
+
+    for groups in (4, 40):
+        case = Case(cuda, 4, "bf16", 128, 64, 32, 1, [100, 40, 64], seed=3)
+        queries = queries_of(case, [8], groups)
+        workspace = attention_workspace(cuda)
+        starts = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+        out, lse = paged_attention(case.pages, case.table, case.lengths, queries, starts(0, 5, 3, 8), workspace, case.flag)
+        assert int(case.flag.item()) == 1 and torch.isfinite(out).all() and torch.isfinite(lse).all()
+        case.flag.zero_()
+        case.lengths[1] = -1
+        out, lse = paged_attention(case.pages, case.table, case.lengths, queries, starts(0, 3, 5, 8), workspace, case.flag)
+        assert int(case.flag.item()) == 1
+        assert (out[3:5] == 0).all() and (lse[3:5] == -math.inf).all() and torch.isfinite(lse[5:]).all()
