@@ -21,6 +21,7 @@ namespace paged {
 constexpr uint32_t kFlagRow = 1;       // a length, row or page id outside the table or the pages
 constexpr uint32_t kFlagPosition = 2;  // a position outside the rotary table
 constexpr uint32_t kFlagTimeout = 4;   // a bounded wait of a kernel ran out
+constexpr uint32_t kFlagShared = 8;    // a kernel's shared memory was not aligned to 1 KB: nothing computed
 
 struct Pages {
   uint8_t *keys;

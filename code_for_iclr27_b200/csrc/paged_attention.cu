@@ -521,7 +521,7 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
   Control<L::kRows> &control = *reinterpret_cast<Control<L::kRows> *>(shared + L::kControlAt);
   volatile int *abort = &control.abort;
   if (base & 1023) {  // the 128-byte swizzle goes by address bits
-    if (threadIdx.x == 0) atomicOr(p.flag, kFlagTimeout);
+    if (threadIdx.x == 0) atomicOr(p.flag, kFlagShared);
     return;
   }
 

@@ -195,7 +195,7 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
   TcControl<L::kTile> &control = *reinterpret_cast<TcControl<L::kTile> *>(shared + L::kControlAt);
   volatile int *abort = &control.abort;
   if (base & 1023) {
-    if (threadIdx.x == 0) atomicOr(p.flag, kFlagTimeout);
+    if (threadIdx.x == 0) atomicOr(p.flag, kFlagShared);
     return;
   }
   const uint32_t scored = shared_address(&control.scored), added = shared_address(&control.added);

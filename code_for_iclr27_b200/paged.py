@@ -202,12 +202,13 @@ class PagedCache:
         self.lengths[:, slots] = 0
 
     def check_flags(self) -> None:
-        """Raise if an operator flagged a row without a place or a position outside its table (a synchronisation)."""
+        """Raise if an operator set a bit of the flag (a synchronisation)."""
         state = int(self.flag.item())
         if state:
             self.flag.zero_()
-            raise RuntimeError(f"paged cache flagged: {state} (1: row outside its pages, 2: position outside the "
-                               "rotary table, 4: a kernel's bounded wait ran out)")
+            raise RuntimeError(f"paged cache flagged: {state} (1: row outside its pages or token of no sequence, "
+                               "2: position outside the rotary table, 4: a kernel's bounded wait ran out, "
+                               "8: a kernel's shared memory was not aligned)")
 
     # ------------------------------------------------------------------ steps
 

@@ -517,7 +517,8 @@ int lrk_arena_evict(const lrk_arena *arena, const int64_t *heads, const float *r
  * page id outside the table or the pages (that row is not touched; a negative
  * length counts as 0) or a token of no sequence, 2 a
  * position outside the rotary table (that token's keys and queries are not
- * written), 4 a bounded wait inside a kernel ran out. */
+ * written), 4 a bounded wait inside a kernel ran out, 8 a kernel's shared memory
+ * was not aligned as it needs (nothing computed). */
 typedef struct lrk_pages {
   void *keys;
   void *values;
