@@ -812,12 +812,22 @@ void arena_append_into(torch::Tensor keys, torch::Tensor values, torch::Tensor p
 
 // ------------------------------------------------------------ paged cache
 
+// The operators have no backward: an input that wants a gradient would lose it
+// without a word.
+void refuse_gradient(const torch::Tensor &tensor) {
+  TORCH_CHECK(!tensor.requires_grad() || !at::GradMode::is_enabled(),
+              "paged operators have no gradient: detach the input that requires one, or call under torch.no_grad()");
+}
+
 // The pages of one cache (lrk_pages): keys, values [pages, page_size, D] of
 // one 16-bit type, or uint8 [pages, page_size, D / 2] with float16 scales
 // [pages, page_size, D / group, 2].
 lrk_pages pages_of(const torch::Tensor &keys, const torch::Tensor &values, const torch::Tensor &positions,
                    const std::optional<torch::Tensor> &key_scales, const std::optional<torch::Tensor> &value_scales) {
-  for (const auto &tensor : {keys, values, positions}) check_cuda(tensor, keys);
+  for (const auto *tensor : {&keys, &values, &positions}) {
+    check_cuda(*tensor, keys);
+    refuse_gradient(*tensor);
+  }
   TORCH_CHECK(keys.dim() == 3 && keys.sizes() == values.sizes() && keys.scalar_type() == values.scalar_type(),
               "pages: keys/values must be [pages, page_size, channels] of one dtype");
   TORCH_CHECK(positions.scalar_type() == at::kFloat && positions.dim() == 2 && positions.size(0) == keys.size(0) &&
@@ -879,6 +889,7 @@ lrk_rows rows_of(const torch::Tensor &tensor, torch::Tensor &copy) {
 
 void check_rows(const torch::Tensor &rows, const torch::Tensor &pages, int64_t dimension, const char *message) {
   TORCH_CHECK(rows.is_cuda() && rows.device() == pages.device(), "CUDA devices differ");
+  refuse_gradient(rows);
   TORCH_CHECK(rows.dim() == 3 && rows.size(1) >= 1 && rows.size(2) == dimension &&
                   (rows.scalar_type() == at::kHalf || rows.scalar_type() == at::kBFloat16),
               message);
@@ -911,6 +922,7 @@ std::optional<torch::Tensor> paged_append(const torch::Tensor &keys, const torch
   TORCH_CHECK(flag.scalar_type() == at::kInt && flag.numel() >= 1, "flag must be int32");
   if (rotary.has_value()) {
     check_cuda(*rotary, keys);
+    refuse_gradient(*rotary);
     TORCH_CHECK(rotary->scalar_type() == at::kFloat && rotary->dim() == 2 && rotary->size(1) >= 1,
                 "rotary table must be float32 [positions, rotary dimension]");
   }

@@ -12,7 +12,8 @@ offset + scale * (code - 8).
 
 PagedCache keeps the pages, tables and lengths of every layer, and moves a request between the packed layout, which
 audits and evictions work on (kvcache.PackedCache), and pages, which decode reads: `load` after an audit, `to_packed`
-before the next one.  No counterpart in the reference, whose attention is FlashAttention over the packed layer
+before the next one.  They have no gradient (a KV cache has no backward pass): inputs that require one are refused outside of torch.no_grad().
+No counterpart in the reference, whose attention is FlashAttention over the packed layer
 (attention.py:15-35) and whose cache is 16-bit (cache.py:16-265).
 """
 from __future__ import annotations

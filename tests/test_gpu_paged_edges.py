@@ -445,3 +445,30 @@ def test_starts_that_descend_and_negative_lengths_are_flagged(cuda):
         out, lse = paged_attention(case.pages, case.table, case.lengths, queries, starts(0, 3, 5, 8), workspace, case.flag)
         assert int(case.flag.item()) == 1
         assert (out[3:5] == 0).all() and (lse[3:5] == -math.inf).all() and torch.isfinite(lse[5:]).all()
+
+
+def test_inputs_that_want_a_gradient_are_refused(cuda):
+    """The operators have no backward: an input that requires a gradient would lose it without a word."""
+    import torch
+
+    from code_for_iclr27_b200.paged import attention_workspace, paged_append, paged_attention, rotary_table
+
+    case = Case(cuda, 16, "bf16", 128, 0, 16, 2, [20, 20])
+    starts, workspace = case.starts([1]), attention_workspace(cuda)
+    q = torch.zeros(1, 4, 128, dtype=torch.bfloat16, device=cuda)
+    k = torch.zeros(1, 2, 128, dtype=torch.bfloat16, device=cuda)
+    position = torch.zeros(1, dtype=torch.int64, device=cuda)
+    rotary = rotary_table(4, 128, 10000.0, cuda)
+    wants = lambda x: x.clone().requires_grad_(True)  # noqa: E731
+    attend = lambda q=q: paged_attention(case.pages, case.table, case.lengths, q, starts, workspace, case.flag)  # noqa: E731
+    append = lambda k=k, v=k, q=q, r=rotary: paged_append(case.pages, case.table, case.lengths, k, v, position, starts, case.flag, r, False, q)  # noqa: E731
+    for call in (lambda: attend(wants(q)), lambda: append(k=wants(k)), lambda: append(v=wants(k)), lambda: append(q=wants(q)),
+                 lambda: append(r=wants(rotary))):
+        with pytest.raises(RuntimeError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+        with torch.inference_mode():
+            call()
+    attend(wants(q).detach())
+    append(wants(k).detach())
