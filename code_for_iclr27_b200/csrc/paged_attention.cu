@@ -661,14 +661,14 @@ void attention_kernel(const __grid_constant__ AttentionParam p, const __grid_con
 #pragma unroll
         for (int step = 1; step < kAcross; step <<= 1)
           largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, step));
-        // A power of two brings the row's largest value into [1, 2): f16 then
-        // holds bf16 values exactly down to 2^-14 of the row's largest, and the
-        // rest to 2^-25 of it.
+        // A power of two brings the row's largest value into [1, 2) ([2, 4) from
+        // 2^127 on): f16 then holds bf16 values exactly down to 2^-14 of the row's
+        // largest, and the rest to 2^-25 of it.
         const int exponent = static_cast<int>(__float_as_uint(largest) >> 23);
         const bool plain = exponent == 255 || largest == 0.0f;
         const int shift = plain ? 0 : (exponent == 0 ? 1 : exponent) - 127;
         const float to_unit = __int_as_float(((127 - min(shift, 126)) << 23) | (turn & 0x80000000u));
-        const float from_unit = __int_as_float((127 + min(shift, 127)) << 23);
+        const float from_unit = __int_as_float((127 + min(shift, 126)) << 23);
         __half h[8];
         float group_sum = 0.0f;
 #pragma unroll

@@ -398,7 +398,7 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
         const bool plain = exponent == 255 || largest == 0.0f;
         const int shift = plain ? 0 : (exponent == 0 ? 1 : exponent) - 127;
         const float to_unit = __int_as_float(((127 - min(shift, 126)) << 23) | (turn & 0x80000000u));
-        const float from_unit = __int_as_float((127 + min(shift, 127)) << 23);
+        const float from_unit = __int_as_float((127 + min(shift, 126)) << 23);
         factor = fmaxf(fabsf(p.scale_log2) * from_unit, kLeastFactor);
         constexpr int kParts = L::kGroups > 1 ? L::kGroups / 2 : 1;  // groups, or the part of one, in half a row
         float part_sums[kParts];

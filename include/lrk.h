@@ -570,6 +570,8 @@ int lrk_paged_append(const lrk_pages *pages, const int32_t *table, int64_t table
  * used.  A NaN key reaches the queries that see its row and no other; a value
  * that is not finite may, in a call of several queries a sequence, also reach
  * those of the slot's queries that do not see its row (0 times NaN).
+ * Over 4-bit rows |scale|, and |scale| times a query's largest channel, have to stay
+ * below 2^106.
  * 16-bit pages and queries share one type.  Sums and softmax statistics are float32;
  * weights are rounded once to f16 (4-bit and f16 rows) or bf16.
  * workspace: lrk_paged_attention_workspace_bytes() bytes, 16-byte aligned,

@@ -472,3 +472,22 @@ def test_inputs_that_want_a_gradient_are_refused(cuda):
             call()
     attend(wants(q).detach())
     append(wants(k).detach())
+
+
+@pytest.mark.parametrize("bits,dtype,dim,group", FOUR_BITS)
+@pytest.mark.parametrize("tokens", [1, 70])
+def test_queries_at_the_ends_of_their_type(cuda, bits, dtype, dim, group, tokens):
+    """bfloat16 queries up to 2^128 and down to its subnormals, with scales that bring their scores back."""
+    import torch
+
+    case = Case(cuda, bits, dtype, dim, group, 32, 1, [200], seed=3)
+    for exponent in (127, 126, 100, -100, -125, -126, -130):
+        queries = queries_of(case, [tokens], 2).double().clamp(-1.9, 1.9)
+        queries[:, :, 0] = 1.75
+        queries = (queries * 2.0 ** exponent).to(torch.bfloat16)
+        assert torch.isfinite(queries).all()
+        scale = case.dim ** -0.5 * 2.0 ** -exponent
+        if scale >= 2.0 ** 100:  # what a scale in float32 holds beside the kernels' own factors
+            scale = 2.0 ** 100
+        out, lse = case.attend(queries, [tokens], scale=scale)
+        compare(case, queries, [tokens], out, lse, scale=float(np.float32(scale)))
