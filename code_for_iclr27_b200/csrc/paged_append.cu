@@ -299,7 +299,10 @@ __global__ __launch_bounds__(kThreads, BY_TOKENS ? (INSIDE ? 5 : 4) : 1) void ap
         store_codes<D, GROUP>(pool, is_key ? p.pages.key_scales : p.pages.value_scales, row, lane, x);
       }
       if (is_key && row >= 0 && lane == 0) p.pages.positions[row] = static_cast<float>(position);
-    } else if (live && !lost && part < parts) {
+    } else if (live && part < parts) {
+      if (lost)  // nothing else says which queries were not rotated
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = __int_as_float(0x7fffffff);
       T *to = static_cast<T *>(p.out_queries) + (token * p.query_heads + (part - 2 * p.heads)) * D + first;
       store8(to, x);
       store8(to + D / 2, x + 8);
@@ -329,7 +332,8 @@ struct ReadParam {
 constexpr int kReadRows = 2;
 
 // D / 16 lanes per row, keys and values of the row together; a lane group takes
-// two neighbouring rows, which mostly share their slot's lookup.
+// two neighbouring rows, which mostly share their slot's lookup.  Rows without a
+// place read as NaN.
 template <typename T, int D, int GROUP, typename S>
 __global__ __launch_bounds__(kThreads) void read_kernel(const ReadParam p) {
   constexpr int kLanes = D / 16, kTeams = kThreads / kLanes;
@@ -356,14 +360,19 @@ __global__ __launch_bounds__(kThreads) void read_kernel(const ReadParam p) {
   if constexpr (GROUP == 0) {
 #pragma unroll
     for (int k = 0; k < kReadRows; ++k) {
-      if (rows[k] < 0) continue;
+      if (row0 + k >= p.rows) continue;
 #pragma unroll
       for (int side = 0; side < 2; ++side) {
         const S *from = reinterpret_cast<const S *>(side ? p.pages.values : p.pages.keys) + rows[k] * D + lane * 8;
         T *to = static_cast<T *>(side ? p.values : p.keys) + (row0 + k) * D + lane * 8;
         float x[16];
-        load8(from, x);
-        load8(from + D / 2, x + 8);
+        if (rows[k] >= 0) {
+          load8(from, x);
+          load8(from + D / 2, x + 8);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] = __int_as_float(0x7fffffff);
+        }
         store8(to, x);
         store8(to + D / 2, x + 8);
       }
@@ -373,6 +382,13 @@ __global__ __launch_bounds__(kThreads) void read_kernel(const ReadParam p) {
     __half2 pairs[kReadRows][2][2];
 #pragma unroll
     for (int k = 0; k < kReadRows; ++k) {
+#pragma unroll
+      for (int side = 0; side < 2; ++side)
+#pragma unroll
+        for (int chunk = 0; chunk < 2; ++chunk) {
+          words[k][side][chunk] = 0;
+          pairs[k][side][chunk] = __halves2half2(__ushort_as_half(0x7fff), __ushort_as_half(0x7fff));
+        }
       if (rows[k] < 0) continue;
 #pragma unroll
       for (int side = 0; side < 2; ++side)
@@ -386,7 +402,7 @@ __global__ __launch_bounds__(kThreads) void read_kernel(const ReadParam p) {
     }
 #pragma unroll
     for (int k = 0; k < kReadRows; ++k) {
-      if (rows[k] < 0) continue;
+      if (row0 + k >= p.rows) continue;
 #pragma unroll
       for (int side = 0; side < 2; ++side)
 #pragma unroll
@@ -406,7 +422,8 @@ __global__ __launch_bounds__(kThreads) void read_kernel(const ReadParam p) {
   }
 #pragma unroll
   for (int k = 0; k < kReadRows; ++k)
-    if (rows[k] >= 0 && lane == 0) p.positions[row0 + k] = p.pages.positions[rows[k]];
+    if (lane == 0 && row0 + k < p.rows)
+      p.positions[row0 + k] = rows[k] >= 0 ? p.pages.positions[rows[k]] : __int_as_float(0x7fffffff);
 }
 
 template <typename T, int D, int GROUP>

@@ -105,7 +105,8 @@ def paged_append(pages: Pages, table, lengths, new_keys, new_values, new_positio
     AFTER the append (left as they are); new_keys, new_values [tokens, heads, D] (any strides); new_positions int64
     [tokens]; token_starts int32 [sequences + 1]: token i of sequence s, of n_s, becomes row lengths - n_s + i of its
     slots.  `rotary` (rotary_table) rotates keys and `queries` [tokens, query heads, D]; the rotated queries are
-    returned.  Rows without a place, and positions outside the table, are left out and set bits of `flag` (int32 [1])."""
+    returned.  Rows without a place, and positions outside the table, are left out (such a token's queries are NaN) and
+    set bits of `flag` (int32 [1])."""
     return _operators().paged_append(pages.keys, pages.values, pages.positions, pages.key_scales, pages.value_scales,
                                     table, lengths, new_keys, new_values, new_positions, token_starts, flag, rotary,
                                     interleaved, queries)
@@ -125,7 +126,8 @@ def paged_attention(pages: Pages, table, lengths, queries, token_starts, workspa
 
 def paged_read(pages: Pages, table, first_rows, row_starts, rows: int, dtype, flag):
     """(keys, values [rows, D] of `dtype`, positions float32 [rows]): of each slot s, row_starts[s + 1] - row_starts[s]
-    rows from first_rows[s] on (both int32; `rows` is row_starts[-1]), back to back."""
+    rows from first_rows[s] on (both int32; `rows` is row_starts[-1]), back to back.  Rows without a place are NaN and set
+    a bit of `flag`."""
     return _operators().paged_read(pages.keys, pages.values, pages.positions, pages.key_scales, pages.value_scales,
                                   table, first_rows, row_starts, rows, dtype, flag)
 

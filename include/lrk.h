@@ -516,8 +516,8 @@ int lrk_arena_evict(const lrk_arena *arena, const int64_t *heads, const float *r
  * The operators OR bits into *flag (device, required): 1 a length, row or
  * page id outside the table or the pages (that row is not touched; a negative
  * length counts as 0) or a token of no sequence, 2 a
- * position outside the rotary table (that token's keys and queries are not
- * written), 4 a bounded wait inside a kernel ran out, 8 a kernel's shared memory
+ * position outside the rotary table (that token's keys are not written, its
+ * rotated queries are NaN), 4 a bounded wait inside a kernel ran out, 8 a kernel's shared memory
  * was not aligned as it needs (nothing computed). */
 typedef struct lrk_pages {
   void *keys;
@@ -587,7 +587,8 @@ int lrk_paged_attention(const lrk_pages *pages, const int32_t *table, int64_t ta
 /* Rows back in the packed layout: row j of slot s's row_starts[s+1] -
  * row_starts[s] rows (i32 [slots + 1], device, from 0 to rows) is the slot's
  * row first_rows[s] + j; keys, values [rows, dimension] of dtype (f16, bf16 or
- * f32: the values that the rows stand for), positions f32 [rows]. */
+ * f32: the values that the rows stand for), positions f32 [rows].  Rows without a
+ * place are NaN. */
 int lrk_paged_read(const lrk_pages *pages, const int32_t *table, int64_t table_stride, int64_t table_width,
                    const int32_t *first_rows, const int32_t *row_starts, int64_t slots, int64_t rows, void *keys,
                    void *values, float *positions, int dtype, unsigned int *flag, lrk_stream_t stream);

@@ -491,3 +491,47 @@ def test_queries_at_the_ends_of_their_type(cuda, bits, dtype, dim, group, tokens
             scale = 2.0 ** 100
         out, lse = case.attend(queries, [tokens], scale=scale)
         compare(case, queries, [tokens], out, lse, scale=float(np.float32(scale)))
+
+
+@pytest.mark.parametrize("bits,dtype,dim,group", [(16, "bf16", 128, 0), (4, "f16", 64, 32)])
+@pytest.mark.parametrize("tokens", [3, 1500])
+def test_queries_without_a_rotation_are_not_numbers(cuda, bits, dtype, dim, group, tokens):
+    """A position outside the rotary table: the token's rotated queries are NaN, not what their memory held."""
+    import torch
+
+    from code_for_iclr27_b200.paged import paged_append, rotary_table
+
+    case = Case(cuda, bits, dtype, dim, group, 64, 1, [tokens], seed=2)
+    rows = queries_of(case, [tokens], 3)
+    position = torch.arange(tokens, device=cuda) % 50
+    position[1], position[2] = 50, -1
+    for rotary_dim in (dim, 32):
+        fill_free_memory(cuda, [rows.numel() * 2])
+        turned = paged_append(case.pages, case.table, case.lengths, rows[:, :1], rows[:, :1], position, case.starts([tokens]),
+                              case.flag, rotary_table(50, rotary_dim, 10000.0, cuda), False, rows)
+        assert int(case.flag.item()) == 2
+        case.flag.zero_()
+        assert torch.isnan(turned[1:3]).all()
+        assert torch.isfinite(turned[0]).all() and torch.isfinite(turned[3:]).all()
+
+
+@pytest.mark.parametrize("bits,dtype,dim,group", [(16, "bf16", 128, 0), (4, "f16", 64, 32)])
+@pytest.mark.parametrize("out", ["f16", "bf16", "f32"])
+def test_rows_read_from_no_page_are_not_numbers(cuda, bits, dtype, dim, group, out):
+    import torch
+
+    from code_for_iclr27_b200.paged import paged_read
+
+    kind = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}[out]
+    case = Case(cuda, bits, dtype, dim, group, 32, 1, [70, 64], seed=2)
+    case.table[0, 1] = -1
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    # Slot 0's rows 0..69 (32..63 have no page), slot 1's rows -2..61, and three rows of no slot.
+    read = lambda: paged_read(case.pages, case.table, ints(0, -2), ints(0, 70, 134), 137, kind, case.flag)  # noqa: E731
+    fill_free_memory(cuda, [137 * dim * kind.itemsize, 137 * 4])
+    keys, values, positions = read()
+    assert int(case.flag.item()) == 1
+    lost = torch.zeros(137, dtype=torch.bool, device=cuda)
+    lost[32:64] = lost[70:72] = lost[134:] = True
+    for got in (keys, values, positions):
+        assert torch.isnan(got[lost]).all() and torch.isfinite(got[~lost]).all()
