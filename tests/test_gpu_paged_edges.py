@@ -9,7 +9,7 @@ import math
 import numpy as np
 import pytest
 
-from test_gpu_paged import FORMATS, UNIT, Case, queries_of
+from test_gpu_paged import APPEND, FORMATS, UNIT, Case, check_append, queries_of, run_append
 
 pytestmark = pytest.mark.gpu
 
@@ -535,3 +535,132 @@ def test_rows_read_from_no_page_are_not_numbers(cuda, bits, dtype, dim, group, o
     lost[32:64] = lost[70:72] = lost[134:] = True
     for got in (keys, values, positions):
         assert torch.isnan(got[lost]).all() and torch.isfinite(got[~lost]).all()
+
+
+@pytest.mark.parametrize("bits,dtype,dim,group", APPEND)
+@pytest.mark.parametrize("rotary,interleaved", [(0, False), (16, True), (32, False), (64, False), (64, True), (128, False), (128, True)])
+@pytest.mark.parametrize("counts,heads,query_heads", [([1000, 0, 37], 3, 5), ([1024], 1, 0), ([7, 1030], 2, 4)])
+def test_append_of_many_tokens(cuda, bits, dtype, dim, group, rotary, interleaved, counts, heads, query_heads):
+    """Over a thousand tokens, not a multiple of what a block takes, with rows (2 heads + query heads) that fill the
+    last four of a block in part: every rotation, bit for bit."""
+    if rotary > dim:
+        pytest.skip("rotates more channels than the head has")
+    before = [(53 * i) % 130 for i in range(len(counts) * heads)]
+    args = run_append(cuda, bits, dtype, dim, group, 32, counts, before, heads, query_heads, rotary, interleaved, rotary != 32)
+    check_append(*args, counts, heads, query_heads, interleaved)
+
+
+@pytest.mark.parametrize("bits,dtype,dim,group", APPEND)
+@pytest.mark.parametrize("rotary", [32, 64])
+def test_append_of_many_tokens_flags_what_has_no_place(cuda, bits, dtype, dim, group, rotary):
+    """Rows beyond the table or in pages that do not exist, and positions outside the rotary table, among 1,100 tokens:
+    their rows stay as they were, the others are written."""
+    import torch
+
+    from code_for_iclr27_b200.paged import paged_append, rotary_table
+
+    tokens = 1100
+    case = Case(cuda, bits, dtype, dim, group, 64, 2, [tokens, tokens - 3], seed=5)
+    case.table[0, 2] = -1
+    case.table[1, 16] = 2 ** 30
+    rows = queries_of(case, [tokens], 1)
+    positions = torch.arange(tokens, device=cuda) % 50
+    positions[700], positions[701], positions[9] = 50, -1, 2 ** 40
+    before = case.pages.positions.clone()
+    # (The second head's first three rows are negative.)
+    paged_append(case.pages, case.table, case.lengths, rows, rows, positions, case.starts([tokens]), case.flag,
+                 rotary_table(50, rotary, 10000.0, cuda), False, None)
+    assert int(case.flag.item()) == 3
+    want = before.cpu()
+    for head, shift in ((0, 0), (1, 3)):
+        for t in range(tokens):
+            row = t - shift
+            if row < 0 or t in (700, 701, 9):
+                continue
+            page = int(case.host_table[head, row // 64])
+            if (head, row // 64) in ((0, 2), (1, 16)):
+                continue
+            want[page, row % 64] = float(t % 50)
+    assert torch.equal(case.pages.positions.cpu(), want)
+
+
+MANY = [(16, "bf16", 128, 0), (16, "f16", 64, 0), (4, "bf16", 128, 32), (4, "f16", 128, 64), (4, "bf16", 128, 128), (4, "f16", 64, 32),
+        (4, "bf16", 64, 64)]
+
+
+@pytest.mark.parametrize("bits,dtype,dim,group", MANY)
+@pytest.mark.parametrize("page", [16, 128])
+def test_chunks_with_peaked_and_large_scores(cuda, bits, dtype, dim, group, page):
+    """Scores of some hundreds: the running maximum moves all the time; a scale of their sign turned round, and zero."""
+    case = Case(cuda, bits, dtype, dim, group, page, 1, [500, 77], seed=2, key_spread=8.0)
+    queries = queries_of(case, [70, 70], 1, spread=8.0)
+    for scale in (None, -0.5, 0.0):
+        out, lse = case.attend(queries, [70, 70], scale=scale)
+        case.check(queries, [70, 70], out, lse, scale=scale)
+
+
+@pytest.mark.parametrize("bits,dtype,dim,group", MANY)
+@pytest.mark.parametrize("large", [60.0, 4000.0, 15000.0])
+def test_chunks_over_values_of_all_magnitudes(cuda, bits, dtype, dim, group, large):
+    for spread in (lambda n: large * (np.arange(n) + 1.0) / max(n, 1), lambda n: np.where(np.arange(n) % 97 == 50, large, 1e-3)):
+        case = Case(cuda, bits, dtype, dim, group, 32, 1, [700, 40], seed=13, value_spread=spread)
+        queries = queries_of(case, [70, 70], 1)
+        out, lse = case.attend(queries, [70, 70])
+        case.check(queries, [70, 70], out, lse)
+
+
+@pytest.mark.parametrize("bits,dtype,dim,group", MANY)
+def test_chunks_of_tiny_and_huge_queries(cuda, bits, dtype, dim, group):
+    case = Case(cuda, bits, dtype, dim, group, 32, 1, [200], seed=3)
+    for factor in (1e-6, 1e-3, 3e4, 0.0) + ((1e30, 1e-30) if dtype == "bf16" else ()):
+        queries = ((queries_of(case, [70], 2).float()).clamp(-2, 2) * factor).to(case.dtype)
+        scale = case.dim ** -0.5 if factor < 1 else case.dim ** -0.5 / factor
+        out, lse = case.attend(queries, [70], scale=scale)
+        case.check(queries, [70], out, lse, scale=scale)
+
+
+@pytest.mark.parametrize("bits,dtype,dim,group", MANY)
+@pytest.mark.parametrize("page", [16, 64])
+def test_chunks_strided_split_and_captured(cuda, bits, dtype, dim, group, page):
+    """Queries as views of a joint projection and of a wider row; slots split over many blocks; a captured call."""
+    import torch
+
+    from code_for_iclr27_b200.paged import attention_workspace, paged_attention
+
+    case = Case(cuda, bits, dtype, dim, group, page, 1, [9001, 300], seed=6)
+    counts = [33, 40]
+    queries = queries_of(case, counts, 4)
+    workspace = attention_workspace(cuda)
+    want, want_lse = case.attend(queries, counts, workspace=workspace)
+    case.check(queries, counts, want, want_lse)
+    joint = torch.zeros(73, 9, dim, dtype=queries.dtype, device=cuda)
+    joint[:, 2:6] = queries
+    odd = torch.zeros(73, 4, dim + 3, dtype=queries.dtype, device=cuda)
+    odd[:, :, 1:1 + dim] = queries
+    for view in (joint[:, 2:6], odd[:, :, 1:1 + dim], queries.transpose(0, 1).contiguous().transpose(0, 1)):
+        out, lse = case.attend(view, counts, workspace=workspace)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    starts = case.starts(counts)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = paged_attention(case.pages, case.table, case.lengths, queries, starts, workspace, case.flag)
+    for _ in range(2):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("bits,dtype,dim,group", MANY)
+def test_a_chunk_over_a_key_that_is_not_a_number(cuda, bits, dtype, dim, group):
+    """It reaches the queries that see its row and no other."""
+    import torch
+
+    case = Case(cuda, bits, dtype, dim, group, 16, 1, [150, 150], seed=8)
+    poison_keys(case, 0, [149 - 20])
+    out, lse = case.attend(queries_of(case, [70, 70], 1), [70, 70])
+    sees = torch.zeros(140, dtype=torch.bool, device=cuda)
+    sees[49:70] = True  # token i of 70 sees rows up to 80 + i
+    assert torch.isnan(out[sees]).all() and torch.isnan(lse[sees]).all()
+    assert torch.isfinite(out[~sees]).all() and torch.isfinite(lse[~sees]).all()
