@@ -136,7 +136,8 @@ class PagedCache:
     """Pages, page tables and lengths of every layer of a batch of sequences; page allocation is on the host.
 
     A step: `advance(counts)` once, then per layer `append` and `attend`.  The step's token_starts and the page tables
-    are shared by every launch of the step."""
+    are shared by every launch of the step, and keep their places: a graph captured of a step's appends and attentions
+    serves later steps of as many tokens, `advance` called before each replay."""
 
     def __init__(self, layers: int, sequences: int, heads: int, dim: int, pages: int, device, dtype=None, bits: int = 16,
                  group: int = 64, page_size: int = 64, max_rows: int = 1 << 17):
@@ -156,6 +157,8 @@ class PagedCache:
         self._free: List[int] = list(range(int(pages) - 1, -1, -1))
         self._held: List[List[List[int]]] = [[[] for _ in range(slots)] for _ in range(self.layers)]
         self._workspaces = {}
+        # The step's token starts and new rows a slot, in place: a captured step finds the next step's there.
+        self._step = torch.zeros(self.sequences + 1 + slots, dtype=torch.int32, device=self.device)
         self.token_starts = None
 
     # ------------------------------------------------------------ allocation
@@ -228,9 +231,10 @@ class PagedCache:
         self.rows += per_slot
         self.seen_tokens += counts
         starts = np.concatenate(([0], np.cumsum(counts)))
-        both = upload(np.concatenate((starts, per_slot)).astype(np.int32), self.device)
-        self.token_starts = both[:self.sequences + 1]
-        self.lengths.add_(both[self.sequences + 1:])
+        staged = torch.from_numpy(np.concatenate((starts, per_slot)).astype(np.int32)).pin_memory()
+        self._step.copy_(staged, non_blocking=True)
+        self.token_starts = self._step[:self.sequences + 1]
+        self.lengths.add_(self._step[self.sequences + 1:])
 
     def append(self, layer: int, new_keys, new_values, positions, rotary=None, interleaved: bool = False, queries=None):
         """The step's rows of one layer (paged_append); returns the rotated queries, if any."""

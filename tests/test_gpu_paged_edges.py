@@ -664,3 +664,55 @@ def test_a_chunk_over_a_key_that_is_not_a_number(cuda, bits, dtype, dim, group):
     sees[49:70] = True  # token i of 70 sees rows up to 80 + i
     assert torch.isnan(out[sees]).all() and torch.isnan(lse[sees]).all()
     assert torch.isfinite(out[~sees]).all() and torch.isfinite(lse[~sees]).all()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_a_captured_step_serves_later_steps(cuda, bits):
+    """A graph of a step's appends and attentions, replayed after each advance (counts shifting between the sequences,
+    new pages among them), gives the bits of the same steps called directly on another cache."""
+    import torch
+
+    from code_for_iclr27_b200.paged import PagedCache, rotary_table
+    from test_gpu_arena import make_packed
+
+    packed = [make_packed(cuda, seed=s) for s in (1, 2)]
+    page_size = 16 if bits == 4 else 64
+    caches = [PagedCache(3, 2, 4, 128, 24 * 1024 // page_size, cuda, bits=bits, page_size=page_size, max_rows=1024)
+              for _ in range(2)]
+    rotary = rotary_table(2000, 128, 10000.0, cuda)
+    joint = torch.zeros(3, 5, 16, 128, dtype=torch.bfloat16, device=cuda)
+    position = torch.zeros(5, dtype=torch.int64, device=cuda)
+
+    def step(cache):
+        outs = []
+        for layer in range(3):
+            q, k, v = joint[layer].split([8, 4, 4], 1)
+            outs.append(cache.attend(layer, cache.append(layer, k, v, position, rotary, queries=q)))
+        return outs
+
+    for cache in caches:
+        for s in range(2):
+            cache.load(s, packed[s])
+    graph = held = None
+    for number, counts in enumerate(([2, 3], [1, 4], [5, 0], [0, 5], [3, 2], [4, 1], [2, 3])):
+        joint.copy_(torch.randn(joint.shape, generator=torch.Generator().manual_seed(number)))
+        position.fill_(900 + number)
+        for cache in caches:
+            cache.advance(counts)
+        want = step(caches[0])
+        if graph is None:
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                held = step(caches[1])
+        fill_free_memory(cuda, [(3 + 8) * 4, 256, 512])  # what a step has let go of is used again
+        graph.replay()
+        torch.cuda.synchronize()
+        for (out, lse), (want_out, want_lse) in zip(held, want):
+            assert torch.isfinite(want_out).all()
+            assert torch.equal(out, want_out) and torch.equal(lse, want_lse)
+    for cache in caches:
+        cache.check_flags()
+    for s in range(2):
+        for a, b in zip(caches[0].to_packed(s).layers, caches[1].to_packed(s).layers):
+            assert torch.equal(a.keys, b.keys) and torch.equal(a.values, b.values) and torch.equal(a.positions, b.positions)
