@@ -314,8 +314,9 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
   // 2^(e - 13), e the larger of the offset's exponent field and the scale's plus 3;
   // the power stays while that is at most 2^(15 + power), and brings it below
   // 2^(11 + power) otherwise (as far as f16 holds 2^-power).  Pairs that are not
-  // finite reach their own rows, whatever the power.
-  const auto tile_power = [&](const uint8_t *stage, uint64_t absent, int32_t power, bool first) {
+  // finite reach their own rows, whatever the power.  `room`: what the pairs' bits
+  // lack to that limit, less than 2^15 each.  Returns the factor for the output so far.
+  const auto tile_power = [&](const uint8_t *stage, uint64_t absent, int32_t &power, uint32_t &room, bool first) {
     constexpr int kWords = L::kTile * L::kGroups / 32;
     uint32_t w[kWords];
     const uint8_t *from = stage + 2 * L::kCodes + L::kScales + lane * kWords * 4;
@@ -326,18 +327,16 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
       const uint2 x = *reinterpret_cast<const uint2 *>(from);
       w[0] = x.x, w[1] = x.y;
     }
-    uint32_t largest = 0;
 #pragma unroll
     for (int k = 0; k < kWords; ++k) w[k] &= 0x7fff7fffu;
     if (absent != 0)
 #pragma unroll
       for (int k = 0; k < kWords; ++k)
         if (absent >> ((lane * kWords + k) / L::kGroups) & 1) w[k] = 0;
+    uint32_t largest = w[0];
 #pragma unroll
-    for (int k = 0; k < kWords; ++k) largest = __vmaxu2(largest, w[k]);
-    const bool passes = (largest & 0xffffu) >= static_cast<uint32_t>(26 + power) << 10 ||
-                        (largest >> 16) >= static_cast<uint32_t>(29 + power) << 10;
-    if (!first && !__any_sync(0xffffffffu, passes)) return power;
+    for (int k = 1; k < kWords; ++k) largest = __vmaxu2(largest, w[k]);
+    if (!first && !__any_sync(0xffffffffu, ((largest + room) & 0x80008000u) != 0)) return 1.0f;
     int32_t field = 0;
 #pragma unroll
     for (int k = 0; k < kWords; ++k) {
@@ -345,7 +344,11 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
       field = max(field, max(scale < 31 ? scale + 3 : 0, offset < 31 ? offset : 0));
     }
     field = __reduce_max_sync(0xffffffffu, field);
-    return max(field - 24, first ? -15 : power);
+    const int32_t last = power;
+    power = max(field - 24, first ? -15 : power);
+    room = static_cast<uint32_t>(max(0x8000 - ((26 + power) << 10), 0)) |
+           static_cast<uint32_t>(max(0x8000 - ((29 + power) << 10), 0)) << 16;
+    return first ? 1.0f : __int_as_float((127 + last - power) << 23);
   };
   const auto waits = [&](uint32_t barrier, uint32_t parity) {
     if (!wait(barrier, parity, abort)) {
@@ -430,6 +433,7 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
     }
     float top = -INFINITY, sum = 0.0f;
     int32_t power = 0;  // 4-bit values are held as v 2^-power
+    uint32_t room = 0;
 
     for (int32_t i = 0; i < tiles; ++i, ++count) {
       const uint32_t slot = count % L::kStages;
@@ -456,9 +460,7 @@ void attention_tc_kernel(const __grid_constant__ AttentionParam p, const __grid_
           reinterpret_cast<float4 *>(shared + L::kTableAt)[k] = make_float4(a.x, b.x, a.y, b.y);
         }
         const uint64_t absent = absent_rows();
-        const int32_t next = tile_power(stage, absent, power, i == 0);
-        if (i > 0) change = __int_as_float((127 + power - next) << 23);
-        power = next;
+        change = tile_power(stage, absent, power, room, i == 0);
         if (i > 0) waits(added, (count - 1) & 1);  // the last tile's values have been used
         unpack_values(stage, absent, power);
       } else {
