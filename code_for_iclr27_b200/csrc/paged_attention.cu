@@ -128,6 +128,13 @@ __device__ __forceinline__ uint32_t pack(const __nv_bfloat16 *, float lo, float 
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// Two halves, 65504 in the place of NaN and what is larger.
+__device__ __forceinline__ uint32_t drop_nan(uint32_t x) {
+  uint32_t y;
+  asm("min.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x7bff7bffu));
+  return y;
+}
+
 template <int WORDS>
 __device__ __forceinline__ void load_words(const uint8_t *from, uint32_t *w) {
   if constexpr (WORDS == 4) {
@@ -412,7 +419,10 @@ struct Consumer {
           }
           b[nt][0] = transpose8(pack(static_cast<const P *>(nullptr), scaled[0], scaled[1]));
           b[nt][1] = transpose8(pack(static_cast<const P *>(nullptr), scaled[2], scaled[3]));
-          mma(static_cast<const P *>(nullptr), scaled_sum[nt][gi / 2], ones, b[nt][0], b[nt][1], scaled_sum[nt][gi / 2]);
+          // A NaN (whose own products reach the group's output) must not reach the other
+          // group through the zeros of `ones`: the minimum drops it.
+          const uint32_t summed[2] = {kNG > 1 ? drop_nan(b[nt][0]) : b[nt][0], kNG > 1 ? drop_nan(b[nt][1]) : b[nt][1]};
+          mma(static_cast<const P *>(nullptr), scaled_sum[nt][gi / 2], ones, summed[0], summed[1], scaled_sum[nt][gi / 2]);
         }
         const uint8_t *at = values_at + gi * (GROUP / 2) + g * (GROUP / 16);
         constexpr int kWords = GROUP == 128 ? 2 : 1;

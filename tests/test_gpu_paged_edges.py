@@ -716,3 +716,26 @@ def test_a_captured_step_serves_later_steps(cuda, bits):
     for s in range(2):
         for a, b in zip(caches[0].to_packed(s).layers, caches[1].to_packed(s).layers):
             assert torch.equal(a.keys, b.keys) and torch.equal(a.values, b.values) and torch.equal(a.positions, b.positions)
+
+
+@pytest.mark.parametrize("dim,group", [(128, 32), (128, 64), (64, 32)])
+@pytest.mark.parametrize("groups", [4, 14, 30, 70])
+@pytest.mark.parametrize("size", [1.0])
+@pytest.mark.parametrize("bad", [0, 1])
+def test_a_value_group_that_is_not_a_number_leaves_the_others_alone(cuda, dim, group, groups, size, bad):
+    """Rows with a group of channels that append held as NaN: those channels are NaN, the others keep compare's bound."""
+    import torch
+
+    rng = np.random.default_rng(7)
+    case = Case(cuda, 4, "bf16", dim, group, 32, 1, [700, 40], seed=13)
+    refill(case, lambda n: (rng.standard_normal((n, dim)), size * rng.standard_normal((n, dim))))
+    queries = queries_of(case, [1, 1], groups)
+    for slot, row in ((0, 3), (0, 650), (1, 39)):
+        case.pages.value_scales[int(case.host_table[slot, row // 32]), row % 32, bad] = float("nan")
+    out, lse = case.attend(queries, [1, 1])
+    at = slice(bad * group, (bad + 1) * group)
+    assert torch.isnan(out[:, :, at]).all() and torch.isfinite(lse).all()
+    out[:, :, at] = 0
+    for slot in range(2):
+        case.rows[slot][1][:, at] = 0
+    compare(case, queries, [1, 1], out, lse)
