@@ -218,12 +218,17 @@ struct Consumer {
     load_words<4>(query_at + ((nt * (D / 32) + pair) * 32 + lane) * 16, b);
   }
 
-  // The largest of the value scales' bits in this lane's row of the tile.
+  // The largest of the value scales' bits, signs left out, in this lane's row of
+  // the tile; with FINITE, of those that are finite.
+  template <bool FINITE = false>
   __device__ __forceinline__ static uint32_t largest_scale(const uint8_t *stage, int lane) {
     uint32_t w[kNG], largest = 0;
     load_words<kNG>(stage + 2 * L::kCodes + L::kScales + lane * L::kScaleBytes, w);
 #pragma unroll
-    for (int gi = 0; gi < kNG; ++gi) largest = max(largest, w[gi] & 0xffffu);
+    for (int gi = 0; gi < kNG; ++gi) {
+      const uint32_t bits = w[gi] & 0x7fffu;
+      largest = max(largest, FINITE && bits >= 0x7c00u ? 0u : bits);
+    }
     return largest;
   }
 
@@ -235,8 +240,7 @@ struct Consumer {
     const int32_t lifted = lift;
     if constexpr (GROUP != 0) {
       if (__any_sync(0xffffffffu, largest > plain_scale())) {
-        // NaN scales (0x7fff) reach their own weights alone, whatever the lift.
-        const uint32_t exponent = __reduce_max_sync(0xffffffffu, largest < 0x7c00u ? largest >> 10 : 0x1eu);
+        const uint32_t exponent = __reduce_max_sync(0xffffffffu, largest >> 10);
         lift = max(lift, static_cast<int32_t>(exponent) - 17);  // scale < 2^(exponent - 14)
       }
     }
@@ -492,7 +496,15 @@ struct Consumer {
         // Also where best is NaN: top has to become NaN, since -inf stands for no rows.
         raises |= !(fmaf(best[nt][i], factor[nt][i], static_cast<float>(lift) - kMost) <= top[nt][i]);
       }
-    if (__any_sync(0xffffffffu, raises)) raise(best, largest);
+    if (__any_sync(0xffffffffu, raises)) {
+      // Scales that are not finite reach their own group, whatever the lift, and must
+      // not cost the others their precision.
+      if constexpr (GROUP != 0) {
+        if (largest >= 0x7c00u) largest = largest_scale<true>(stage, lane);
+        __syncwarp();
+      }
+      raise(best, largest);
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

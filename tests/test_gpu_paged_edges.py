@@ -720,7 +720,7 @@ def test_a_captured_step_serves_later_steps(cuda, bits):
 
 @pytest.mark.parametrize("dim,group", [(128, 32), (128, 64), (64, 32)])
 @pytest.mark.parametrize("groups", [4, 14, 30, 70])
-@pytest.mark.parametrize("size", [1.0])
+@pytest.mark.parametrize("size", [1.0, 1e-6])
 @pytest.mark.parametrize("bad", [0, 1])
 def test_a_value_group_that_is_not_a_number_leaves_the_others_alone(cuda, dim, group, groups, size, bad):
     """Rows with a group of channels that append held as NaN: those channels are NaN, the others keep compare's bound."""
