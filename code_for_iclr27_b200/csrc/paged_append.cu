@@ -17,12 +17,14 @@
 // bf16's 8 bits would move the ends of the range by up to a third of one.
 //
 // Memory bounds both (every row read and written once), launches the small ones.
-// Measured: 19,538 tokens of 8 + 8 + 32 heads into 16-bit pages 87 us, 5.6 TB/s
-// of what has to move; 32,768 tokens into 4-bit pages and the rows back 199 us,
-// 4.5 TB/s (the quantiser costs some ten instructions a channel); one layer of
-// 276,000 4-bit rows back in bf16 34.6 us, 5.3 TB/s.  With 16 neighbouring
-// channels a lane, so that half of every rotated pair was read twice and half a
-// sector stored at a time, the three took 109, 267 and 38 us.
+// Measured: 19,538 tokens of 8 + 8 + 32 heads into 16-bit pages 88 us, 5.6 TB/s
+// of what has to move; 32,768 tokens into 4-bit pages and the rows back 207 us,
+// 4.4 TB/s (the append at 58 % of the issue slots, waiting for its rows most; the
+// quantiser costs some ten instructions a channel); one layer of 276,000 4-bit rows
+// back in bf16 37.5 us, 4.9 TB/s, at 73 % of the integer pipe.  In short runs the
+// three took 87, 199 and 34.6 us, and with 16 neighbouring channels a lane, so that
+// half of every rotated pair was read twice and half a sector stored at a time, 109,
+// 267 and 38 us.
 #include "paged.cuh"
 
 namespace lrk {

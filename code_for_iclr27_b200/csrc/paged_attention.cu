@@ -11,10 +11,11 @@
 // query head, so memory bounds it if the 4-bit codes can be unpacked as fast
 // as they arrive: at the copy rate about 40 codes per SM and clock, three
 // instructions per code.  Measured (32 requests of 33,768 rows a head, 8 query
-// heads a KV head, group 128): 257 us, 4.57 TB/s, 70 % of the copy rate, at 60 %
-// of the issue slots and of the integer pipe; copies alone, with nothing
-// computed, 203 us.  In 16 bits (8 ragged requests) 5.6 TB/s.  Hence the shape
-// of the arithmetic:
+// heads a KV head, group 128): 268 to 285 us by machine, 4.1 to 4.4 TB/s, 63 to
+// 67 % of the copy rate, at 58 % of the issue slots and 60 % of the integer pipe
+// (four warps a scheduler wait for their own instructions); copies alone, with
+// nothing computed, 203 us.  In 16 bits (8 ragged requests) 58 to 60 us, 5.4 TB/s.
+// Hence the shape of the arithmetic:
 //
 // * S^T = K Q^T and O^T = V^T P^T on m16n8k16 matrix instructions with the
 //   cache as the 16-row operand A, straight from registers, and the (few)
@@ -35,9 +36,9 @@
 // Tiles are 32 rows; every warp moves its own (bulk copies, or TMA boxes with a
 // 128-byte swizzle for 16-bit rows) into one or two stages of its own, so the
 // warps of a block meet only at a unit's ends.  How the tiles are split over the
-// blocks: paged_attention.cuh.  Measured on the way: a feeding warp per block
-// (16 consumers and 4 feeders an SM) 296 us; twenty warps at 96 registers, with
-// spills, 276; sixteen at 128 registers 257.
+// blocks: paged_attention.cuh.  Measured on the way, in short runs of the long
+// case: a feeding warp per block (16 consumers and 4 feeders an SM) 296 us; twenty
+// warps at 96 registers, with spills, 276; sixteen at 128 registers 257.
 #include <cuda.h>
 
 #include <algorithm>

@@ -73,6 +73,8 @@ __device__ __forceinline__ uint32_t shared_address(const void *p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
+// 2^x to a relative 2^-22 or so; results below 2^-126 are 0.
+// The weights are rounded to 11 or 8 bits after it.
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -21,11 +21,12 @@
 // operand with channels contiguous (MN-major), so nothing is transposed.
 //
 // Measured (250 tokens of 32 query heads over 8 slots of 34,768 rows, group 64):
-// 381 us, 373 TFLOP/s, 23 % of the matrix peak; the tensor pipe is busy a fifth
-// of the time and half the issue slots are used, by unpacking, by the scales (two
+// 404 us, 352 TFLOP/s, 21 % of the matrix peak; the tensor pipe is busy a fifth
+// of the time and 45 % of the issue slots are used, by unpacking, by the scales (two
 // packed multiply-adds per pair of scores and group) and by the exponentials,
-// between three barriers a tile.  The same work on paged_attention.cu's matrix
-// instructions took 765 us.
+// between three barriers a tile.  (With a fixed power for the values, and rows
+// without a page not told apart, 391 us.)  The same work on paged_attention.cu's
+// matrix instructions took 765 us.
 //
 // Two blocks run on an SM (256 tensor-memory columns and at most 113 KB each)
 // and fill one another's waits; within a block the value product of a tile runs

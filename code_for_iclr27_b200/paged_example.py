@@ -5,7 +5,8 @@
 A synthetic request's packed cache is audited and evicted (audit.audit_pass), its surviving rows go into pages
 (PagedCache.load), decode steps append the new token's rotated, quantised rows and attend over the pages, and the rows
 come back into the packed layout (to_packed) for the next audit.  The same steps on 16-bit pages, on the same inputs,
-show what 4 bits cost.  Returns (and prints) the bytes a row takes, the time of a step and how far the outputs are off.
+show what 4 bits cost.  Returns (and prints) the bytes a row takes, the device's time of a step's appends and attentions
+(the host's page allocation, PagedCache.advance, comes before it) and how far the outputs are off.
 """
 from __future__ import annotations
 
