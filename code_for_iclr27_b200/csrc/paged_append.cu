@@ -34,9 +34,9 @@ using namespace paged;
 
 constexpr int kThreads = 128;
 // From here on append_kernel goes BY_TOKENS (8 KV, 32 query heads, D = 128, into
-// 16-bit pages; into 4-bit pages and back): 512 tokens 5.6 and 11.5 us against 4.5
-// and 9.6, 1,024 6.8 and 13.5 against 6.5 and 13.4, 2,048 10.7 and 17.5 against
-// 11.7 and 21.3.
+// 16-bit pages; into 4-bit pages and back): 512 tokens 5.4 and 11.4 us against 4.5
+// and 9.7, 1,024 6.0 and 13.5 against 6.5 and 13.4, 2,048 10.3 and 17.5 against
+// 11.8 and 21.4.
 constexpr int kManyTokens = 1024;
 
 struct AppendParam {

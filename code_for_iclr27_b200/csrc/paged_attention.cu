@@ -58,9 +58,9 @@ constexpr int kTile = 32;   // rows per tile
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 // More query rows a slot than this go to paged_attention_tc.cu.  At 64 rows this
-// file's kernel takes 54, 82 and 40 us (one request of 16,384 rows a head,
-// D = 128; 24 of 4,000, D = 64; two of 8,192 in 16 bits) and that one 59, 99 and
-// 44; at 96 rows 68, 115 and 57 against 72, 107 and 51.
+// file's kernel takes 54, 84 and 41 us (one request of 16,384 rows a head,
+// D = 128; 24 of 4,000, D = 64; two of 8,192 in 16 bits) and that one 62, 103 and
+// 45; at 96 rows 68, 120 and 58 against 72, 112 and 52.
 constexpr int kMatrixRows = 64;
 constexpr int kMinTiles = kWarps;  // tiles per block, at least
 constexpr int kCrossing = 10;      // a second unit's cost in tiles: its start, its end, its join
